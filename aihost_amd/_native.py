@@ -25,6 +25,7 @@ HIP_ERROR_OUT_OF_MEMORY = 2
 F32, Q4_0, Q8_0, Q4_K, Q6_K = 0, 2, 8, 12, 14
 F16_IEEE, F16_REFCPU = 0, 1
 PRE_NONE, PRE_RMSNORM, PRE_SILU_MUL, PRE_SILU_PAIRS, PRE_F16_OPERAND = 0, 1, 2, 3, 4
+KV_INT8, KV_E4M3 = 0, 1
 POST_STORE, POST_ACCUMULATE, POST_SILU_PAIRS, POST_SILU_PAIRS_F16 = 0, 1, 2, 3
 
 
@@ -45,8 +46,36 @@ class DeviceInfo(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """aih_kv_cache: a paged 8-bit KV cache in device memory."""
+    _fields_ = [
+        ("format", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_tokens", ctypes.c_int32),
+        ("n_blocks", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class KvScores(ctypes.Structure):
+    """aih_kv_scores: what changes the scores of aih_kv_attention."""
+    _fields_ = [
+        ("cap", ctypes.c_float),
+        ("window", ctypes.c_int32),
+        ("slopes", ctypes.c_void_p),
+        ("prefix", ctypes.c_void_p),
+    ]
+
+
 _vp, _i, _i64, _u64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_size_t
 _f, _fp = ctypes.c_float, ctypes.POINTER(ctypes.c_float)
+
+_i32, _kvp, _scp = ctypes.c_int32, ctypes.POINTER(KvCache), ctypes.POINTER(KvScores)
 
 # name -> (restype, argtypes); the full exported surface of the header
 SIGNATURES = {
@@ -101,6 +130,15 @@ SIGNATURES = {
                                       ctypes.c_int32, _vp, _vp, ctypes.c_int32, ctypes.c_int32, _f, _vp, _i64]),
     "aih_embed_q": (_i, [_vp, _i, _vp, _i64, _i64, _vp, _i64, _vp]),
     "aih_argmax": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, ctypes.c_int32]),
+    "aih_kv_cache_bytes": (_i64, [_kvp]),
+    "aih_kv_plan": (_i, [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "aih_kv_release": (_i, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "aih_kv_append": (_i, [_vp, _kvp, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "aih_kv_append_rope": (_i, [_vp, _kvp, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i32]),
+    "aih_kv_read": (_i, [_vp, _kvp, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "aih_kv_attention_scratch_floats": (_i64, [_vp, _kvp, _i32, _i64, _i32, _i32]),
+    "aih_kv_attention": (_i, [_vp, _kvp, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _f, _scp, _vp,
+                              _i64]),
     "aih_sync": (_i, [_vp]),
     "aih_stream": (_vp, [_vp]),
     "aih_capture_begin": (_i, [_vp]),
@@ -142,6 +180,13 @@ def lib():
 
 def strerror(status):
     return lib().aih_strerror(int(status)).decode()
+
+
+def check_size(n, what):
+    """A size that the library returned; raises for a negative status."""
+    if n < 0:
+        raise AihError(int(n), what)
+    return int(n)
 
 
 def operand_bytes(m, k):

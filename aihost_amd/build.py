@@ -32,9 +32,10 @@ HIP_FLAGS = [
 # the decoder operators round their element-wise formulas like the reference;
 # the batch-1/2 matvec writes its fused multiply-adds out, so that every
 # activation column is computed by the same instructions (and its fused
-# prologues round like the separate decoder operators).
+# prologues round like the separate decoder operators); the KV cache's rotated
+# keys round like aih_rope's.
 EXTRA = {"aih_dequant.hip": ["-ffp-contract=off"], "aih_decoder.hip": ["-ffp-contract=off"],
-         "aih_qmatvec.hip": ["-ffp-contract=off"]}
+         "aih_qmatvec.hip": ["-ffp-contract=off"], "aih_kv_cache.hip": ["-ffp-contract=off"]}
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-pthread"]
 
 

@@ -1,0 +1,790 @@
+// aih_kv_attention.hip -- grouped-query attention over the paged 8-bit KV cache
+// (include/aihost_hip.h), for single tokens, a few tokens and prompts.
+//
+// Products.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16.  The
+// codes (integers up to 127, or e4m3 numbers) are exact in fp16; q and the
+// probabilities are split into two fp16 values of 22 bits together, so a
+// product is two MFMAs and the result is good to fp32: rounding either to one
+// fp16 would leave about 1e-4.  The scales stay out of the products: a lane's 16
+// scores of a 64-key tile belong to one group of 16 tokens, hence to one block,
+// so the key scale is one factor of the lane and the value scale one factor of
+// its probabilities.
+//
+// Layouts (lane l, c = l % 16, g = l / 16): A[i][k] lane i + 16 (k/8) element
+// k % 8, B[k][j] lane j + 16 (k/8) element k % 8, D[i][j] lane j + 16 (i/4)
+// register i % 4.  A tile is four groups of 16 tokens.
+//   S^T product t = 0..3: row i = 4a + b of A is key 16a + 4t + b of the tile,
+//     so that D gives lane (c, g) the scores of query c with keys 16g + 4t + b.
+//     The 16 bytes that lane (c, g) loads of a key are dimensions 64 C + 16 g ..
+//     of it; their halves are the k-slots of two MFMAs, and Q is laid out alike.
+//   O^T product (16 dimensions dt, half m): k-slot 8g + j is key 16g + 8m + j,
+//     so P is the lane's own registers 8m + j and V the halves of the 16
+//     bytes (one dimension, 16 tokens) that lane (c, g) loads from group g.
+// The cache's layout is made for these loads: no byte moves between lanes.
+//
+// Softmax.  In base 2, with the running normalizer, sum and accumulator of each
+// query in the registers of the four lanes that hold it.  A weight is the
+// probability times the value scale, so the normalizer M is taken over both:
+// with t the score and e the exponent of the scale, M is max(t + e) over the keys seen
+// so far, rounded up.  p = 2^(t + e - M) is at most 1, the weight
+// p vs 2^(15 - e) at most 2^15, the accumulator holds O 2^15 2^-M and the
+// sum 2^-M of the probabilities' (each p 2^-e).  M and e being integers,
+// rescaling is exact, and rare.  e is held within 60 of the largest exponent that
+// the query has met (a smaller scale's values are below fp32's last bit
+// beside those, and the sum must not lose the probability of a block of zeros),
+// and above -100; blocks that a query does not see do not enter its M.
+//
+// Work.  Rows are (token, head of the group) pairs of one KV head, token-major,
+// in tiles of R; each tile's keys are split into parts where the tiles alone
+// would leave CUs idle or where one request is much longer than the others.
+// Every workgroup finds its part from the lengths (find_item), so a captured
+// launch follows the requests as they grow.
+
+#include "aih_kv.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace {
+
+using aih_kv::f4;
+using aih_kv::u4;
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kNone = 0xFFFFFFFFu;   // no group of tokens there
+
+struct Args {
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    const float *Q;
+    float *O;
+    int64_t ldq, ldo;
+    const int32_t *starts, *lens, *tables;
+    const float *slopes;
+    const int32_t *prefix;
+    float *part, *part_ml;      // partial outputs (rows of D floats) and their (maximum, sum)
+    int32_t rows, heads, group, n_seqs, width, n_blocks, shift, window;
+    int32_t target, least;      // workgroups wanted; the fewest tiles of a part
+    int32_t n_part;             // partial tiles that fit the scratch
+    float scale, cap;
+};
+
+// ---------------------------------------------------------------- which part is mine
+struct Seq {
+    int32_t start, n, len;   // first query row, query rows, cached tokens
+};
+
+__device__ __forceinline__ Seq seq_of(const Args &a, int s)
+{
+    const int32_t b = min(max(a.starts[s], 0), a.rows), e = min(max(a.starts[s + 1], b), a.rows);
+    const int64_t most = (int64_t)a.width << a.shift;
+    return Seq{b, e - b, (int32_t)min<int64_t>(max(a.lens[s], 0), most)};
+}
+
+// Row tiles of R rows of a request, and the key tiles that the longest of them spans.
+template <int R>
+__device__ __forceinline__ int32_t row_tiles(const Args &a, const Seq &q)
+{
+    return (int32_t)(((int64_t)q.n * a.group + R - 1) / R);
+}
+__device__ __forceinline__ int32_t key_tiles(const Args &a, const Seq &q)
+{
+    const int32_t lo = a.window > 0 ? max(0, q.len - q.n + 1 - a.window) : 0;
+    return (int32_t)(((int64_t)q.len + 63) / 64) - lo / 64;
+}
+
+struct Item {
+    int32_t seq, tile, split, n_split, part;   // part: index of the tile's first partial (n_split > 1)
+    Seq q;
+    bool ok;
+};
+
+template <typename T>
+__device__ __forceinline__ T wave_add(T v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Item `idx` of one KV head: parts are numbered request by request, tile by
+// tile (the last, longest one first), split by split; with `joined`, tiles
+// instead.  Part length: the whole work over the wanted workgroups, so that
+// all parts are about as long whatever the requests' lengths.  Every wave of
+// the launch runs this with all lanes.
+template <int R>
+__device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t heads, bool joined)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t work = 0;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const int s = base + lane;
+        if (s < a.n_seqs) {
+            const Seq q = seq_of(a, s);
+            work += (int64_t)row_tiles<R>(a, q) * max(key_tiles(a, q), 0);
+        }
+    }
+    work = wave_add(work) * heads;
+    const int32_t len = (int32_t)max<int64_t>(a.least, (work + a.target - 1) / a.target);
+    int32_t before = 0, parts = 0;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const int s = base + lane;
+        Seq q{0, 0, 0};
+        int32_t tiles = 0, n_split = 1;
+        if (s < a.n_seqs) {
+            q = seq_of(a, s);
+            tiles = row_tiles<R>(a, q);
+            n_split = max(1, (key_tiles(a, q) + len - 1) / len);
+        }
+        const int32_t own = joined ? tiles : tiles * n_split;
+        int32_t upto = own, part_upto = n_split > 1 ? tiles * n_split : 0;
+        const int32_t part_own = part_upto;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int32_t o = __shfl_up(upto, d), p = __shfl_up(part_upto, d);
+            if (lane >= d) {
+                upto += o;
+                part_upto += p;
+            }
+        }
+        const unsigned long long past = __ballot(before + upto > idx);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            Item it;
+            const int32_t k = idx - (before + __builtin_amdgcn_readlane(upto - own, l));
+            it.n_split = __builtin_amdgcn_readlane(n_split, l);
+            const int32_t nt = __builtin_amdgcn_readlane(tiles, l);
+            it.tile = joined ? k : nt - 1 - k / it.n_split;
+            it.split = joined ? 0 : k % it.n_split;
+            it.seq = base + l;
+            it.part = parts + __builtin_amdgcn_readlane(part_upto - part_own, l) + it.tile * it.n_split;
+            it.q = Seq{__builtin_amdgcn_readlane(q.start, l), __builtin_amdgcn_readlane(q.n, l),
+                       __builtin_amdgcn_readlane(q.len, l)};
+            it.ok = true;
+            return it;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+        parts += __builtin_amdgcn_readlane(part_upto, 63);
+    }
+    Item none{};
+    none.ok = false;
+    return none;
+}
+
+// The key tiles of a row tile, and of its part `split`: an equal share each.
+struct Range {
+    int32_t lo, hi;
+};
+
+template <int R>
+__device__ __forceinline__ Range tile_keys(const Args &a, const Item &it)
+{
+    const int64_t f0 = (int64_t)it.tile * R, f1 = min<int64_t>(f0 + R, (int64_t)it.q.n * a.group) - 1;
+    const int32_t base = it.q.len - it.q.n;
+    const int32_t p0 = base + (int32_t)(f0 / a.group), p1 = base + (int32_t)(f1 / a.group);
+    int32_t end = p1 + 1;
+    if (a.prefix) end = max(end, a.prefix[it.seq]);
+    end = min(end, it.q.len);
+    const int32_t lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+    return Range{lo / 64, end <= lo ? lo / 64 : (int32_t)(((int64_t)end + 63) / 64)};
+}
+
+__device__ __forceinline__ Range part_of(const Range &r, int32_t split, int32_t n_split)
+{
+    const int32_t per = (r.hi - r.lo + n_split - 1) / n_split;
+    const int32_t lo = min(r.lo + split * per, r.hi);
+    return Range{lo, min(lo + per, r.hi)};
+}
+
+// ---------------------------------------------------------------- codes to fp16
+template <int FMT>
+__device__ __forceinline__ h8 to_half(uint32_t w0, uint32_t w1);
+
+// A code + 128 below an exponent byte is 1024 + 128 + code; the subtraction is exact.
+template <>
+__device__ __forceinline__ h8 to_half<AIH_KV_INT8>(uint32_t w0, uint32_t w1)
+{
+    w0 ^= 0x80808080u;
+    w1 ^= 0x80808080u;
+    constexpr uint32_t e = 0x64646464u;
+    const u4 b = {__builtin_amdgcn_perm(w0, e, 0x00050004u), __builtin_amdgcn_perm(w0, e, 0x00070006u),
+                  __builtin_amdgcn_perm(w1, e, 0x00050004u), __builtin_amdgcn_perm(w1, e, 0x00070006u)};
+    return __builtin_bit_cast(h8, b) - (_Float16)1152.0f;
+}
+
+template <>
+__device__ __forceinline__ h8 to_half<AIH_KV_E4M3>(uint32_t w0, uint32_t w1)
+{
+    const u4 b = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true))};
+    return __builtin_bit_cast(h8, b);
+}
+
+// x0, x1 = hi + lo, two pairs of fp16
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo)
+{
+    const f2 x = {x0, x1};
+    const h2 h = __builtin_convertvector(x, h2);
+    const h2 l = __builtin_convertvector(x - __builtin_convertvector(h, f2), h2);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+__device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Over the four lanes c, c + 16, c + 32, c + 48 of a query.
+__device__ __forceinline__ float over4_max(float v)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float over4_sum(float v)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// tanh to fp32: the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...)))
+// cut after the fifth level below 0.7 (relative error under 3e-9 there), 1 - 2 / (e^2x + 1) above.
+__device__ __forceinline__ float tanh_small(float x)
+{
+    const float y = x * x;
+    const float n = fmaf(fmaf(y, 1.0f, 105.0f), y, 945.0f), d = fmaf(fmaf(y, 15.0f, 420.0f), y, 945.0f);
+    return x * n * __builtin_amdgcn_rcpf(d);
+}
+__device__ __forceinline__ float tanh_any(float x)
+{
+    const float a = fabsf(x);
+    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * a);
+    const float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    return a < 0.7f ? tanh_small(x) : copysignf(t, x);
+}
+
+// ---------------------------------------------------------------- a query's state
+constexpr float kNoExp = -1000.0f;   // no value scale seen yet
+
+// x 2^d for the difference d of two normalizers (-inf, or NaN for two of those: 0)
+__device__ __forceinline__ float times2(float x, float d) { return ldexpf(x, (int)fmaxf(d, -1000.0f)); }
+
+// 16 queries of a wave: lane (c, g) holds query c's.
+template <int D>
+struct State {
+    f4 o[D / 16];   // rows 16 dt + 4 g + i of O^T, times 2^(15 - M)
+    float m, l;     // M; this lane's part of the sum, times 2^-M
+    float e;        // the largest exponent of a value scale seen
+    __device__ __forceinline__ void init()
+    {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY;
+        l = 0.f;
+        e = kNoExp;
+    }
+    __device__ __forceinline__ void times(float f)
+    {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i] *= f;
+    }
+};
+
+// The query of a column: its place among the rows and what it sees.
+struct Col {
+    int32_t token, head;   // query row (of Q and O), head; token -1: none
+    int32_t pos, lo, hi;   // position; keys lo .. hi - 1 are seen
+    float slope;           // of its head, times log2 e
+};
+
+__device__ __forceinline__ Col column(const Args &a, const Item &it, int32_t kvh, int64_t f)
+{
+    Col c{-1, 0, 0, 0, 0, 0.f};
+    if (f < (int64_t)it.q.n * a.group) {
+        const int32_t i = (int32_t)(f / a.group);
+        c.token = it.q.start + i;
+        c.head = kvh * a.group + (int32_t)(f % a.group);
+        c.pos = it.q.len - it.q.n + i;
+        c.hi = c.pos + 1;
+        if (a.prefix) c.hi = max(c.hi, a.prefix[it.seq]);
+        c.hi = min(c.hi, it.q.len);
+        c.lo = a.window > 0 ? max(0, c.pos - a.window + 1) : 0;
+        if (a.slopes) c.slope = a.slopes[c.head] * kLog2e;
+    }
+    return c;
+}
+
+// Q of a column, split; returns the factor that undoes the split's power of two.
+template <int D>
+__device__ __forceinline__ float load_q(const Args &a, const Col &c, int g, h8 (*qh)[2], h8 (*ql)[2])
+{
+    f4 x[D / 64][4];
+    float mx = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[k][i] = f4{0.f, 0.f, 0.f, 0.f};
+            if (c.token >= 0)
+                x[k][i] = *reinterpret_cast<const f4 *>(a.Q + (int64_t)c.token * a.ldq + c.head * D + 64 * k + 16 * g + 4 * i);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fabsf(x[k][i][u]));
+        }
+    mx = over4_max(mx);
+    const int e = 15 - __builtin_amdgcn_frexp_expf(mx);   // the largest |q| into [2^14, 2^15)
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 v = x[k][2 * m + i / 2];
+                split2(ldexpf(v[2 * (i % 2)], e), ldexpf(v[2 * (i % 2) + 1], e), h[i], l[i]);
+            }
+            qh[k][m] = __builtin_bit_cast(h8, u4{h[0], h[1], h[2], h[3]});
+            ql[k][m] = __builtin_bit_cast(h8, u4{l[0], l[1], l[2], l[3]});
+        }
+    return ldexpf(1.0f, -e);
+}
+
+// 64 groups of 16 tokens of a request from key tile t0 on, lane l the l-th:
+// its place in the cache (in groups; kNone past `end` tokens or outside the
+// cache) and its scales.
+struct Groups {
+    uint32_t at;
+    float ks, vs;
+};
+
+__device__ __forceinline__ Groups load_groups(const Args &a, int32_t seq, int32_t len, int32_t kvh, int32_t heads,
+                                              int32_t t0)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t token = ((int64_t)t0 * 4 + lane) * 16;
+    Groups r{kNone, 0.f, 0.f};
+    if (token < len) {
+        const int32_t id = a.tables[(int64_t)seq * a.width + (token >> a.shift)];
+        if (id >= 0 && id < a.n_blocks) {
+            const uint32_t block = (uint32_t)id * (uint32_t)heads + (uint32_t)kvh;
+            r.at = (block << (a.shift - 4)) + (uint32_t)((token & ((1 << a.shift) - 1)) >> 4);
+            r.ks = a.ks[block];
+            r.vs = a.vs[block];
+        }
+    }
+    return r;
+}
+
+// What a lane needs of its group of a tile.
+struct Lane {
+    float ks, vs;   // scales
+    bool none;      // the group is not there
+};
+
+// Scores of a tile to split weights, and the state's normalizer, sum and
+// accumulator brought up to it.  s: the lane's 16 products of query c with keys
+// key0 + 0..15 (key0 = 64 tile + 16 g); f: the factor that makes them scores,
+// times log2 e unless MOD.  HIDE: some key of the tile is not seen by some query.
+template <int D, bool MOD, bool HIDE>
+__device__ __forceinline__ void softmax_tile(const Args &a, const Col &c, const Lane &ln, int32_t key0, float f,
+                                             f4 *s, State<D> &st, h8 *ph, h8 *pl)
+{
+    if constexpr (MOD) {
+        float top = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(s[t][i]));
+        if (a.cap > 0.f) {
+            const float u = f / a.cap, out = a.cap * kLog2e;
+            if (__any(!(top * fabsf(u) < 0.7f))) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][i] = out * tanh_any(s[t][i] * u);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][i] = out * tanh_small(s[t][i] * u);
+            }
+        } else {
+            f *= kLog2e;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[t] *= f;
+        }
+        const float far = (float)(c.pos - key0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = fmaf(-c.slope, fabsf(far - (float)(4 * t + i)), s[t][i]);
+        f = 1.0f;
+    }
+    bool some = true;   // the query sees a key of this lane's group
+    if constexpr (HIDE) {
+        const int32_t lo = c.lo - key0, hi = ln.none ? -1 : c.hi - key0;
+        some = lo < 16 && hi > 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int32_t j = 4 * t + i;
+                s[t][i] = j >= lo && j < hi ? s[t][i] * f : -INFINITY;
+            }
+        f = 1.0f;
+    }
+    const float ve = ln.vs > 0.f && ln.vs < INFINITY ? (float)__builtin_amdgcn_frexp_expf(ln.vs) : kNoExp;
+    st.e = fmaxf(st.e, over4_max(some ? ve : kNoExp));
+    const float e = st.e == kNoExp ? 0.f : fmaxf(fmaxf(ve, st.e - 60.f), -100.f);
+    const float vs = ldexpf(ln.vs, 15 - (int)e);
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+    if constexpr (!MOD && !HIDE) {
+        // beyond 2^20 the rounding of a score is no longer small beside 1: the normalizer and the exponents below have to
+        // come from the same rounded scores
+        if (__any(mx * f > 0x1p20f)) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[t] *= f;
+            mx *= f;
+            f = 1.0f;
+        }
+    }
+    const float m = fmaxf(st.m, ceilf(over4_max(fmaf(mx, f, e))));   // f >= 0; a NaN score is left out here and shows below
+    if (__any(m > st.m)) {
+        const float back = times2(1.0f, st.m - m);
+        st.l *= back;
+        st.times(back);
+        st.m = m;
+    }
+    const float add = e - (m == -INFINITY ? 0.f : m);
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 2 * h + i / 2, u = 2 * (i % 2);
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][u], f, add)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][u + 1], f, add));
+            sum += p0;
+            sum += p1;
+            float w0 = p0 * vs, w1 = p1 * vs;
+            if constexpr (HIDE) {   // a hidden key's block may have no number for a scale
+                w0 = s[t][u] == -INFINITY ? 0.f : w0;
+                w1 = s[t][u + 1] == -INFINITY ? 0.f : w1;
+            }
+            split2(w0, w1, hi[i], lo[i]);
+        }
+        ph[h] = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
+        pl[h] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
+    }
+    st.l += ldexpf(sum, -(int)e);
+}
+
+// ---------------------------------------------------------------- few rows: 16 at a time
+// Workgroup (head fastest): a part of one tile of 16 rows; its four waves take
+// a quarter of the part's keys each, straight from memory to the matrix cores,
+// and join through LDS.
+template <int FMT, int D, bool MOD>
+__global__ void __launch_bounds__(256)
+few_kernel(Args a, int32_t heads)
+{
+    constexpr int C = D / 64, DT = D / 16;
+    __shared__ float os[4][16][D + 4];
+    __shared__ float ms[4][16], ls[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int32_t kvh = blockIdx.x % heads;
+    const Item it = find_item<16>(a, blockIdx.x / heads, heads, false);
+    if (!it.ok) return;
+    const Range all = tile_keys<16>(a, it), mine = part_of(all, it.split, it.n_split);
+    const int32_t nt = mine.hi - mine.lo;
+    const int32_t t0 = mine.lo + nt * w / 4, t1 = mine.lo + nt * (w + 1) / 4;
+
+    const Col col = column(a, it, kvh, (int64_t)it.tile * 16 + c);
+    h8 qh[C][2], ql[C][2];
+    const float undo = load_q<D>(a, col, g, qh, ql) * a.scale * (MOD ? 1.0f : kLog2e);
+    // what every (real) query of the wave sees
+    int32_t see_lo = col.token >= 0 ? col.lo : 0, see_hi = col.token >= 0 ? col.hi : 0x7FFFFFFF;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        see_lo = max(see_lo, __shfl_xor(see_lo, d));
+        see_hi = min(see_hi, __shfl_xor(see_hi, d));
+    }
+
+    State<D> st;
+    st.init();
+    Groups gr{kNone, 0.f, 0.f};
+    for (int32_t t = t0; t < t1; ++t) {
+        const int in = (t - t0) & 15;
+        if (in == 0) gr = load_groups(a, it.seq, it.q.len, kvh, heads, t);
+        const uint32_t at_k = __shfl(gr.at, 4 * in + (c >> 2)), at_v = __shfl(gr.at, 4 * in + g);
+        Lane ln;
+        ln.ks = __shfl(gr.ks, 4 * in + g);
+        ln.vs = __shfl(gr.vs, 4 * in + g);
+        ln.none = at_v == kNone;
+        const uint8_t *kp = a.k + (size_t)(at_k == kNone ? 0 : at_k) * (16 * D) + ((c & 3) * 4 + g) * 16;
+        const uint8_t *vp = a.v + (size_t)(at_v == kNone ? 0 : at_v) * (16 * D) + c * 16;
+        u4 kr[4][C], vr[DT];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < C; ++k) kr[q][k] = *reinterpret_cast<const u4 *>(kp + (q * C + k) * 256);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const u4 *>(vp + d * 256);
+        f4 s[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            s[q] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < C; ++k)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const h8 x = to_half<FMT>(kr[q][k][2 * m], kr[q][k][2 * m + 1]);
+                    s[q] = mfma(x, qh[k][m], s[q]);
+                    s[q] = mfma(x, ql[k][m], s[q]);
+                }
+        }
+        h8 ph[2], pl[2];
+        const int32_t key0 = t * 64 + 16 * g;
+        const bool hide = t * 64 < see_lo || (int64_t)t * 64 + 64 > see_hi || __any(ln.none);
+        if (hide) softmax_tile<D, MOD, true>(a, col, ln, key0, undo * ln.ks, s, st, ph, pl);
+        else softmax_tile<D, MOD, false>(a, col, ln, key0, undo * ln.ks, s, st, ph, pl);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const h8 x = to_half<FMT>(vr[d][2 * m], vr[d][2 * m + 1]);
+                st.o[d] = mfma(x, ph[m], st.o[d]);
+                st.o[d] = mfma(x, pl[m], st.o[d]);
+            }
+    }
+    // join the waves
+    const float l = over4_sum(st.l);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f4 *>(&os[w][c][16 * d + 4 * g]) = st.o[d];
+    if (g == 0) {
+        ms[w][c] = st.m;
+        ls[w][c] = l;
+    }
+    __syncthreads();
+    const int row = tid >> 4;
+    float m = ms[0][row];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = fmaxf(m, ms[i][row]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += times2(ls[i][row], ms[i][row] - m);
+    const bool whole = it.n_split == 1;
+    const Col out = column(a, it, kvh, (int64_t)it.tile * 16 + row);
+    const int32_t part = (it.part + it.split) * heads + kvh;
+    if (!whole && part >= a.n_part) return;   // never: the scratch is sized for every part
+    const float div = !whole ? 1.0f : sum != 0.f ? 0x1p-15f / sum : 0.f;
+    float *to = whole ? a.O + (int64_t)out.token * a.ldo + out.head * D : a.part + ((int64_t)part * 16 + row) * D;
+    if (!whole && (tid & 15) == 0) {
+        a.part_ml[((int64_t)part * 16 + row) * 2] = m;
+        a.part_ml[((int64_t)part * 16 + row) * 2 + 1] = sum;
+    }
+    if (out.token < 0) return;
+#pragma unroll
+    for (int d = 4 * (tid & 15); d < D; d += 64) {
+        f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f4 y = *reinterpret_cast<const f4 *>(&os[i][row][d]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] += times2(y[u], ms[i][row] - m);
+        }
+        *reinterpret_cast<f4 *>(to + d) = x * div;
+    }
+}
+
+// ---------------------------------------------------------------- join the parts
+// Workgroup (head fastest): the rows of one row tile that was split, 16 at a
+// time; thread (row, 16 lanes) takes D / 16 of a row's floats.
+template <int D, int R>
+__global__ void __launch_bounds__(256)
+join_kernel(Args a, int32_t heads)
+{
+    const int tid = threadIdx.x;
+    const int32_t kvh = blockIdx.x % heads;
+    const Item it = find_item<R>(a, blockIdx.x / heads, heads, true);
+    if (!it.ok || it.n_split == 1 || (it.part + it.n_split - 1) * heads + kvh >= a.n_part) return;
+    const Range all = tile_keys<R>(a, it);
+    const int32_t n = all.hi - all.lo, per = (n + it.n_split - 1) / it.n_split;
+    const int32_t parts = per ? (n + per - 1) / per : 0;   // the others are empty
+    for (int r0 = 0; r0 < R; r0 += 16) {
+        const int row = r0 + (tid >> 4);
+        const Col out = column(a, it, kvh, (int64_t)it.tile * R + row);
+        if (out.token < 0) continue;
+        float m = -INFINITY;
+        for (int p = 0; p < parts; ++p)
+            m = fmaxf(m, a.part_ml[((int64_t)((it.part + p) * heads + kvh) * R + row) * 2]);
+        f4 x[D / 64];
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) x[d] = f4{0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+        for (int p = 0; p < parts; ++p) {
+            const int64_t at = (int64_t)((it.part + p) * heads + kvh) * R + row;
+            const float d2 = a.part_ml[at * 2] - m;
+            sum += times2(a.part_ml[at * 2 + 1], d2);
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d) {
+                const f4 y = *reinterpret_cast<const f4 *>(a.part + at * D + 64 * d + 4 * (tid & 15));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[d][u] += times2(y[u], d2);
+            }
+        }
+        const float div = sum != 0.f ? 0x1p-15f / sum : 0.f;
+        float *to = a.O + (int64_t)out.token * a.ldo + out.head * D + 4 * (tid & 15);
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) *reinterpret_cast<f4 *>(to + 64 * d) = x[d] * div;
+    }
+}
+
+// ---------------------------------------------------------------- how a call is split
+// Rows per tile, workgroups wanted, fewest key tiles of a part.
+struct Plan {
+    int rows, least;
+    int64_t target, tiles, items, parts;   // bounds over one KV head (tiles, items) and over all (parts)
+};
+
+Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs,
+             int32_t table_width)
+{
+    const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256, heads = kv->n_kv_heads, group = n_heads / heads;
+    Plan p{};
+    p.rows = 16;
+    p.least = 4;
+    p.target = 4 * cus;
+    const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
+    p.tiles = std::min<int64_t>(n_seqs, rows) + rows * group / p.rows;   // sum of ceil(n_s group / R) over the n_s > 0
+    const int64_t most_split = (most_keys + p.least - 1) / p.least;
+    // sum of tiles * ceil(keys / length) <= tiles + work / length, work / length <= target / heads
+    p.items = std::min(p.tiles * most_split, p.tiles + (p.target + heads - 1) / heads);
+    // a tile that is split has more keys than one part, so its parts are at most twice its keys over the length
+    p.parts = most_split <= 1 ? 0 : std::min(p.items * heads, 2 * p.target);
+    return p;
+}
+
+constexpr int64_t kAlign = 4;   // floats: the partial outputs start on 16 bytes
+
+int64_t ml_floats(const Plan &p) { return (p.parts * p.rows * 2 + kAlign - 1) / kAlign * kAlign; }
+
+template <int FMT, int D, bool MOD>
+int launch(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
+{
+    hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), dim3((unsigned)(p.items * heads)), dim3(256), 0, ctx->stream, a, heads);
+    if (p.parts) {
+        const int rc = aih_launch_status();
+        if (rc) return rc;
+        hipLaunchKernelGGL((join_kernel<D, 16>), dim3((unsigned)(p.tiles * heads)), dim3(256), 0, ctx->stream, a, heads);
+    }
+    return aih_launch_status();
+}
+
+template <int FMT, int D>
+int launch_mod(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
+{
+    return a.cap > 0.f || a.slopes ? launch<FMT, D, true>(ctx, a, p, heads) : launch<FMT, D, false>(ctx, a, p, heads);
+}
+
+template <int FMT>
+int launch_dim(aih_ctx *ctx, int32_t dim, const Args &a, const Plan &p, int32_t heads)
+{
+    switch (dim) {
+    case 64: return launch_mod<FMT, 64>(ctx, a, p, heads);
+    case 128: return launch_mod<FMT, 128>(ctx, a, p, heads);
+    default: return launch_mod<FMT, 256>(ctx, a, p, heads);
+    }
+}
+
+int check_batch(const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs, int32_t table_width)
+{
+    if (n_heads <= 0 || rows < 0 || n_seqs <= 0 || table_width <= 0 || n_heads % kv->n_kv_heads) return AIH_E_INVALID;
+    if (n_seqs > aih_kv::kMaxSeqs || (int64_t)table_width * kv->block_tokens > 0x7FFFFFFF || rows > 0x7FFFFFFF ||
+        rows * n_heads > (int64_t)1 << 33 || n_heads > 1 << 20)
+        return AIH_E_LIMIT;
+    return AIH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t aih_kv_attention_scratch_floats(aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows,
+                                        int32_t n_seqs, int32_t table_width)
+{
+    if (!ctx) return AIH_E_INVALID;
+    int rc = aih_kv::check_shape(kv);
+    if (!rc) rc = check_batch(kv, n_heads, rows, n_seqs, table_width);
+    if (rc) return rc;
+    const Plan p = plan_of(ctx, kv, n_heads, rows, n_seqs, table_width);
+    return ml_floats(p) + p.parts * p.rows * kv->head_dim;
+}
+
+int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64_t ldq, float *O, int64_t ldo,
+                     int64_t rows, int32_t n_heads, int32_t n_seqs, const int32_t *starts, const int32_t *lens,
+                     const int32_t *tables, int32_t table_width, float scale, const aih_kv_scores *scores,
+                     float *scratch, int64_t scratch_floats)
+{
+    if (!ctx) return AIH_E_INVALID;
+    int rc = aih_kv::check_cache(kv);
+    if (!rc) rc = check_batch(kv, n_heads, rows, n_seqs, table_width);
+    if (rc) return rc;
+    const int64_t wide = (int64_t)n_heads * kv->head_dim;
+    if (!Q || !O || !starts || !lens || !tables || ldq < wide || ldo < wide || ldq % 4 || ldo % 4 ||
+        !aih_kv::aligned16(Q) || !aih_kv::aligned16(O) || !(scale > 0.0f) || !std::isfinite(scale))
+        return AIH_E_INVALID;
+    const aih_kv_scores none{};
+    if (!scores) scores = &none;
+    if (!(scores->cap >= 0.0f) || !std::isfinite(scores->cap) || scores->window < 0) return AIH_E_INVALID;
+    const Plan p = plan_of(ctx, kv, n_heads, rows, n_seqs, table_width);
+    const int64_t need = ml_floats(p) + p.parts * p.rows * kv->head_dim;
+    if (need && (!scratch || !aih_kv::aligned16(scratch) || scratch_floats < need)) return AIH_E_INVALID;
+    if (rows == 0) return AIH_OK;
+    if (p.items * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
+    Args a{};
+    a.k = static_cast<const uint8_t *>(kv->k);
+    a.v = static_cast<const uint8_t *>(kv->v);
+    a.ks = kv->k_scale;
+    a.vs = kv->v_scale;
+    a.Q = Q;
+    a.O = O;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.starts = starts;
+    a.lens = lens;
+    a.tables = tables;
+    a.slopes = scores->slopes;
+    a.prefix = scores->prefix;
+    a.part_ml = scratch;
+    a.part = scratch + ml_floats(p);
+    a.rows = (int32_t)rows;
+    a.heads = n_heads;
+    a.group = n_heads / kv->n_kv_heads;
+    a.n_seqs = n_seqs;
+    a.width = table_width;
+    a.n_blocks = kv->n_blocks;
+    a.shift = aih_kv::log2_of(kv->block_tokens);
+    a.window = scores->window;
+    a.target = (int32_t)p.target;
+    a.least = p.least;
+    a.n_part = (int32_t)p.parts;
+    a.scale = scale;
+    a.cap = scores->cap;
+    aih_kv::DeviceGuard guard(ctx->device);
+    AIH_TRY(guard.status);
+    return kv->format == AIH_KV_INT8 ? launch_dim<AIH_KV_INT8>(ctx, kv->head_dim, a, p, kv->n_kv_heads)
+                                     : launch_dim<AIH_KV_E4M3>(ctx, kv->head_dim, a, p, kv->n_kv_heads);
+}
+
+}  // extern "C"

@@ -1,0 +1,732 @@
+// aih_kv_cache.hip -- the bookkeeping and the storing side of the paged 8-bit
+// KV cache (include/aihost_hip.h): block tables and slot maps from request
+// lengths, new rows into the cache with a scale per block and head, and the
+// cache's values back as fp32 rows.  The reading side is aih_kv_attention.hip.
+//
+// This file is compiled without FMA contraction, so that rotated keys round
+// like aih_rope's; the one fused multiply-add that the rounding of a quotient
+// needs is written out.
+
+#include "aih_kv.h"
+
+#include <algorithm>
+
+namespace {
+
+using aih_kv::f4;
+using aih_kv::kMaxSeqs;
+using aih_kv::u4;
+
+// ---------------------------------------------------------------- block tables and slot maps
+// Sums of counts that stop at kFull: the largest value they are compared with
+// is a 31-bit count, and a sum that has stopped is above it or equal.  (Stopped
+// addition of non-negative numbers is associative, so it can be scanned.)
+constexpr uint32_t kFull = 0x7FFFFFFFu;
+
+__device__ __forceinline__ uint32_t add_full(uint32_t a, uint32_t b) { return min(a + b, kFull); }
+
+// Inclusive scan of v over the 1024 threads of a workgroup, and the total.
+// red: 17 words of LDS, free again after the next barrier that follows.
+__device__ __forceinline__ uint32_t scan_1024(uint32_t v, uint32_t *red, uint32_t &total)
+{
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(v, d);
+        if (lane >= d) v = add_full(v, o);
+    }
+    __syncthreads();   // the last use of red
+    if (lane == 63) red[w] = v;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (i == w) before = total;
+        total = add_full(total, red[i]);
+    }
+    return add_full(v, before);
+}
+
+// The request of row r: the last s with starts[s] <= r (starts ascending,
+// starts[n] > r >= starts[0] = 0).
+__device__ __forceinline__ int request_of(const int32_t *starts, int n, int32_t r)
+{
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (starts[mid] <= r) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+struct PlanArgs {
+    const int32_t *lens, *n_new;
+    int32_t *tables;
+    const int32_t *free_blocks, *n_free;
+    int32_t *new_lens, *new_n_free, *starts, *slots, *positions, *refused;
+    int32_t n_seqs, width, shift, n_blocks, rows;
+};
+
+// Slot and position of row r, from the finished plan.  starts may be LDS or global.
+__device__ __forceinline__ void place_row(const PlanArgs &a, const int32_t *starts, const int32_t *new_lens, int32_t r)
+{
+    int32_t slot = -1, pos = -1;
+    if (r < starts[a.n_seqs]) {
+        const int s = request_of(starts, a.n_seqs, r);
+        pos = new_lens[s] - (starts[s + 1] - r);
+        const int32_t id = a.tables[(int64_t)s * a.width + (pos >> a.shift)];
+        if (id >= 0 && id < a.n_blocks) slot = (id << a.shift) + (pos & ((1 << a.shift) - 1));
+    }
+    a.slots[r] = slot;
+    a.positions[r] = pos;
+}
+
+// One workgroup: two rounds of scans over the requests (blocks needed and rows
+// asked for, then rows granted), the handed-out blocks, and, with `place`,
+// the rows.  Latency is all there is to it at the sizes of a decode step: 64
+// requests read 512 bytes.
+__global__ void __launch_bounds__(1024)
+plan_kernel(PlanArgs a, int place)
+{
+    __shared__ int32_t starts[kMaxSeqs + 1];
+    __shared__ uint32_t upto[kMaxSeqs];    // blocks handed out up to and with request s
+    __shared__ int32_t had[kMaxSeqs];      // its blocks before; its new length in the end
+    __shared__ uint32_t red[17];
+    __shared__ int32_t n_refused;
+    const int tid = threadIdx.x;
+    const int32_t bt = 1 << a.shift;
+    const uint32_t n_free = (uint32_t)min(max(*a.n_free, 0), a.n_blocks);
+    if (tid == 0) n_refused = 0;
+    uint32_t need_before = 0, asked_before = 0, rows_before = 0, taken = 0;
+    for (int base = 0; base < a.n_seqs; base += 1024) {
+        const int s = base + tid;
+        int32_t len = 0, n = 0;
+        bool ok = s < a.n_seqs;
+        if (ok) {
+            len = a.lens[s];
+            n = a.n_new[s];
+        }
+        const bool valid = len >= 0 && n >= 0 && (int64_t)len + n <= (int64_t)a.width << a.shift;
+        const int32_t blocks = valid ? (int32_t)(((int64_t)len + bt - 1) >> a.shift) : 0;
+        uint32_t need = valid ? (uint32_t)((((int64_t)len + n + bt - 1) >> a.shift) - blocks) : 0u;
+        uint32_t total;
+        const uint32_t need_upto = add_full(scan_1024(need, red, total), need_before);
+        need_before = add_full(need_before, total);
+        const uint32_t asked = add_full(scan_1024(valid ? (uint32_t)n : 0u, red, total), asked_before);
+        asked_before = add_full(asked_before, total);
+        const bool fits = n == 0 || ((need == 0 || need_upto <= n_free) && asked <= (uint32_t)a.rows);
+        if (ok && !(valid && fits)) atomicAdd(&n_refused, 1);
+        ok = ok && valid && fits;
+        if (!ok) {
+            n = 0;
+            need = 0;
+        }
+        // granted requests that need blocks come before refused ones that do, so their sums are exact
+        const uint32_t begin = add_full(scan_1024((uint32_t)n, red, total), rows_before) - (uint32_t)n;
+        rows_before = add_full(rows_before, total);
+        (void)scan_1024(need, red, total);
+        taken += total;
+        if (s < a.n_seqs) {
+            starts[s] = (int32_t)begin;
+            had[s] = blocks;
+            upto[s] = need ? need_upto : 0u;
+            a.new_lens[s] = len + n;
+        }
+    }
+    if (tid == 0) starts[a.n_seqs] = (int32_t)rows_before;
+    __syncthreads();
+    for (int s = tid; s <= a.n_seqs; s += 1024) a.starts[s] = starts[s];
+    if (tid == 0) {
+        *a.new_n_free = (int32_t)(n_free - taken);
+        *a.refused = n_refused;
+    }
+    // The blocks: request s takes upto[s] - need .. upto[s] - 1 of the order; need from the lengths.
+    for (int s0 = (tid >> 6) * 64; s0 < a.n_seqs; s0 += 1024) {
+        // one wave, 64 requests: lane l looks at request s0 + l, the wave writes each one's entries together
+        const int s = s0 + (tid & 63);
+        int32_t need = 0, first = 0, at = 0;
+        if (s < a.n_seqs && upto[s]) {
+            at = had[s];
+            need = (int32_t)(((int64_t)a.new_lens[s] + bt - 1) >> a.shift) - at;
+            first = (int32_t)upto[s] - need;
+        }
+        unsigned long long some = __ballot(need > 0);
+        while (some) {
+            const int l = __builtin_ctzll(some);
+            some &= some - 1;
+            const int32_t k = __shfl(need, l), f = __shfl(first, l), t = __shfl(at, l);
+            int32_t *to = a.tables + (int64_t)(s0 + l) * a.width + t;
+            for (int j = tid & 63; j < k; j += 64) to[j] = a.free_blocks[(int32_t)n_free - 1 - (f + j)];
+        }
+    }
+    if (!place) return;
+    __syncthreads();
+    for (int s = tid; s < a.n_seqs; s += 1024) had[s] = a.new_lens[s];
+    __syncthreads();
+    for (int32_t r = tid; r < a.rows; r += 1024) place_row(a, starts, had, r);
+}
+
+// The rows of a plan, where they are too many for its one workgroup.
+__global__ void __launch_bounds__(256)
+place_kernel(PlanArgs a)
+{
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256)
+        place_row(a, a.starts, a.new_lens, (int32_t)r);
+}
+
+__global__ void __launch_bounds__(1024)
+release_kernel(int32_t *lens, int32_t n_seqs, int32_t *tables, int32_t width, int32_t shift, int32_t n_blocks,
+               const int32_t *done, int32_t *free_blocks, int32_t *n_free)
+{
+    __shared__ uint32_t first[kMaxSeqs];   // a request's blocks; then where they go on the stack
+    __shared__ uint32_t red[17];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t had = (uint32_t)min(max(*n_free, 0), n_blocks);
+    auto blocks_of = [&](int s) {
+        if (done && !done[s]) return 0;
+        const int64_t b = ((int64_t)max(lens[s], 0) + (1 << shift) - 1) >> shift;
+        return (int32_t)min(b, (int64_t)width);
+    };
+    auto valid = [&](int32_t id) { return id >= 0 && id < n_blocks; };
+    for (int s = w; s < n_seqs; s += 16) {   // one wave counts a request's entries
+        const int32_t n = blocks_of(s);
+        uint32_t c = 0;
+        for (int j = 0; j < n; j += 64)
+            c += (uint32_t)__popcll(__ballot(j + lane < n && valid(tables[(int64_t)s * width + min(j + lane, n - 1)])));
+        if (lane == 0) first[s] = c;
+    }
+    __syncthreads();
+    uint32_t before = 0, total;
+    for (int base = 0; base < n_seqs; base += 1024) {
+        const int s = base + tid;
+        const uint32_t c = s < n_seqs ? first[s] : 0u;
+        const uint32_t up = add_full(scan_1024(c, red, total), before);
+        before = add_full(before, total);
+        if (s < n_seqs) first[s] = up - c;
+    }
+    __syncthreads();
+    for (int s = w; s < n_seqs; s += 16) {
+        const int32_t n = blocks_of(s);
+        uint32_t at = add_full(had, first[s]);
+        for (int j = 0; j < n; j += 64) {
+            int32_t *entry = tables + (int64_t)s * width + min(j + lane, n - 1);
+            const int32_t id = *entry;
+            const bool is = j + lane < n && valid(id);
+            const unsigned long long all = __ballot(is);
+            const uint32_t to = at + (uint32_t)__popcll(all & ((1ull << lane) - 1));
+            if (is && to < (uint32_t)n_blocks) free_blocks[to] = id;
+            if (j + lane < n) *entry = -1;
+            at += (uint32_t)__popcll(all);
+        }
+        if (lane == 0 && (!done || done[s])) lens[s] = 0;
+    }
+    __syncthreads();
+    if (tid == 0) *n_free = (int32_t)min(add_full(had, before), (uint32_t)n_blocks);
+}
+
+// ---------------------------------------------------------------- the formats
+template <int FMT>
+struct Format;
+
+template <>
+struct Format<AIH_KV_INT8> {
+    static constexpr float kMost = 127.0f;
+    // amax / 127, at least the smallest normal number
+    __device__ static __forceinline__ float first_scale(float amax) { return fmaxf(amax / 127.0f, 0x1p-126f); }
+    // The code nearest to x / s, ties to even.  x * inv is within 2^-16 of the
+    // quotient, so c is right or, beside a tie, off by one; r = x - c s is
+    // exact (its bits fit: a multiple of the smaller ulp, at most about s / 2),
+    // and 2 r against s says which.
+    __device__ static __forceinline__ int code(float x, float s, float inv)
+    {
+        float c = __builtin_rintf(x * inv);
+        const float r2 = 2.0f * __builtin_fmaf(-c, s, x);
+        const bool odd = ((int)c & 1) != 0;
+        if (r2 > s || (r2 == s && odd)) c += 1.0f;
+        else if (r2 < -s || (r2 == -s && odd)) c -= 1.0f;
+        return (int)fminf(fmaxf(c, -127.0f), 127.0f);
+    }
+    // four codes into a word
+    __device__ static __forceinline__ uint32_t pack(const float *x, float s, float inv)
+    {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (uint32_t)(code(x[i], s, inv) & 0xFF) << (8 * i);
+        return w;
+    }
+    // the codes of a word times f = 2^-d, rounded
+    __device__ static __forceinline__ uint32_t shrink(uint32_t w, float f)
+    {
+        uint32_t o = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o |= (uint32_t)((int)__builtin_rintf((float)(int8_t)(w >> (8 * i)) * f) & 0xFF) << (8 * i);
+        return o;
+    }
+    __device__ static __forceinline__ float value(uint32_t byte) { return (float)(int8_t)byte; }
+};
+
+template <>
+struct Format<AIH_KV_E4M3> {
+    static constexpr float kMost = 448.0f;
+    // the smallest power of two s with amax <= 448 s = 0.875 2^9 s
+    __device__ static __forceinline__ float first_scale(float amax)
+    {
+        const float m = __builtin_amdgcn_frexp_mantf(amax);   // [0.5, 1)
+        const int e = __builtin_amdgcn_frexp_expf(amax);
+        return ldexpf(1.0f, max(e - (m <= 0.875f ? 9 : 8), -126));
+    }
+    // x / s is exact (s a power of two, 1 / s too) up to what lies far below the smallest code
+    __device__ static __forceinline__ uint32_t pack(const float *x, float s, float inv)
+    {
+        (void)s;
+        int w = 0;
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, w, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, w, true);
+        return (uint32_t)w;
+    }
+    __device__ static __forceinline__ uint32_t shrink(uint32_t v, float f)
+    {
+        const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)v, 0), __builtin_amdgcn_cvt_f32_fp8((int)v, 1),
+                            __builtin_amdgcn_cvt_f32_fp8((int)v, 2), __builtin_amdgcn_cvt_f32_fp8((int)v, 3)};
+        return pack(x, 0.0f, f);
+    }
+    __device__ static __forceinline__ float value(uint32_t byte) { return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0); }
+};
+
+// ---------------------------------------------------------------- append
+struct AppendArgs {
+    uint8_t *k, *v;
+    float *ks, *vs;
+    const float *K, *V;
+    int64_t ldk, ldv;
+    const int32_t *slots;
+    int64_t rows;
+    int32_t heads, n_blocks, shift;   // KV heads; log2 of block_tokens
+    // the rotation: table null for none
+    float *Q;
+    int64_t ldq;
+    const int32_t *positions;
+    const float *table;
+    int32_t table_rows, q_heads, q_parts;
+};
+
+// Two rotation pairs of a row at position p, dimensions d .. d + 3 (d % 4 == 0) of its head.
+template <int D>
+__device__ __forceinline__ f4 rotate(const f4 x, const float *__restrict__ table, int32_t p, int d)
+{
+    const f4 cs = *reinterpret_cast<const f4 *>(table + (int64_t)p * D + d);   // cos, sin of pairs d / 2 and d / 2 + 1
+    return f4{x[0] * cs[0] - x[1] * cs[1], x[0] * cs[1] + x[1] * cs[0], x[2] * cs[2] - x[3] * cs[3],
+              x[2] * cs[3] + x[3] * cs[2]};
+}
+
+// The scale of a block for new values of largest magnitude `top` (bits of
+// |x|), and the power of two d that its present codes are divided by.
+struct Scale {
+    float s, inv;
+    int d;
+};
+
+template <int FMT>
+__device__ __forceinline__ Scale next_scale(uint32_t top, float old, bool fresh)
+{
+    typedef Format<FMT> F;
+    Scale o{fresh ? 0.0f : old, 0.0f, 0};
+    const float amax = __uint_as_float(top);
+    if (top >= 0x7F800000u || o.s != o.s) {
+        o.s = __uint_as_float(0x7FC00000u);
+        return o;
+    }
+    if (top != 0 && o.s == 0.0f) o.s = F::first_scale(amax);
+    else if (top != 0) {
+        const double most = (double)F::kMost * (double)o.s;   // exact
+        if ((double)amax > most) {
+            // the smallest d with amax <= most 2^d: the quotient's exponent, less one where it is a power of two (a
+            // quotient of 24 by 31 bits that is none stays further from it than fp64 rounds)
+            const double q = (double)amax / most;
+            int e;
+            const double m = frexp(q, &e);
+            o.d = m > 0.5 ? e : e - 1;
+            o.s = ldexpf(o.s, o.d);
+        }
+    }
+    if (o.s != 0.0f) o.inv = 1.0f / o.s;
+    return o;
+}
+
+// Workgroup (x, y): KV head y and the runs of rows of one block that begin
+// among rows RPW x .. RPW x + RPW - 1; y past the KV heads: the queries of
+// those rows.  A run's values are read twice, for their largest magnitude and
+// to be rounded; the second time they come from the caches.  Every 16-byte
+// unit of the block belongs to one thread, which reads what it keeps of it
+// (rescaled where the scale grew) and writes it once.
+template <int FMT, int D, bool ROPE>
+__global__ void __launch_bounds__(256)
+append_kernel(AppendArgs a, int rpw)
+{
+    typedef Format<FMT> F;
+    constexpr int NQ = D / 4, C = D / 64;
+    __shared__ int32_t row_of[256];      // the row (from the run's first) whose token is at an offset of the block
+    __shared__ uint32_t top[2][4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t r0 = (int64_t)blockIdx.x * rpw;
+    auto placed = [&](int64_t r) {   // the position of row r allows it to be stored
+        if constexpr (!ROPE) return true;
+        const int32_t p = a.positions[r];
+        return p >= 0 && p < a.table_rows;
+    };
+    if (ROPE && (int)blockIdx.y >= a.heads) {
+        const int per = a.q_heads * NQ;
+        for (int64_t r = r0; r < min(r0 + rpw, a.rows); ++r) {
+            if (!placed(r)) continue;
+            const int32_t p = a.positions[r];
+            for (int i = ((int)blockIdx.y - a.heads) * 256 + tid; i < per; i += a.q_parts * 256) {
+                f4 *q = reinterpret_cast<f4 *>(a.Q + r * a.ldq + 4 * i);
+                *q = rotate<D>(*q, a.table, p, 4 * (i % NQ));
+            }
+        }
+        return;
+    }
+    const int head = blockIdx.y, bt = 1 << a.shift;
+    auto block_of = [&](int64_t r) {   // the block of row r, -1 for none
+        const int32_t slot = a.slots[r];
+        const int32_t b = slot < 0 ? -1 : slot >> a.shift;
+        return b < a.n_blocks ? b : -1;
+    };
+    // which of the rows r0 .. begin a run (rpw <= 64; the same in every wave)
+    bool begins = false;
+    if (lane < rpw && r0 + lane < a.rows) {
+        const int64_t r = r0 + lane;
+        const int32_t b = block_of(r);
+        begins = b >= 0 && (r == 0 || block_of(r - 1) != b);
+    }
+    unsigned long long runs = __ballot(begins);
+    while (runs) {
+        const int64_t r = r0 + __builtin_ctzll(runs);
+        runs &= runs - 1;
+        const int32_t block = block_of(r);
+        // the run: rows r .. r + n - 1
+        int64_t n = 1;
+        for (;;) {
+            const int64_t q = r + n + lane;
+            const unsigned long long other = __ballot(q >= a.rows || block_of(min(q, a.rows - 1)) != block);
+            if (other) {
+                n += __builtin_ctzll(other);
+                break;
+            }
+            n += 64;
+        }
+        const int64_t at = (int64_t)block * a.heads + head;
+        const float old_k = a.ks[at], old_v = a.vs[at];
+        __syncthreads();   // the LDS of the run before
+        row_of[tid] = -1;
+        __syncthreads();
+        for (int64_t j = tid; j < n; j += 256)
+            if (placed(r + j)) atomicMax(&row_of[a.slots[r + j] & (bt - 1)], (int32_t)min<int64_t>(j, 0x7FFFFFFF));
+        const float *K = a.K + r * a.ldk + head * D, *V = a.V + r * a.ldv + head * D;
+        auto key4 = [&](int64_t j, int d) {
+            f4 x = *reinterpret_cast<const f4 *>(K + j * a.ldk + d);
+            if constexpr (ROPE) x = rotate<D>(x, a.table, a.positions[r + j], d);
+            return x;
+        };
+        uint32_t tk = 0, tv = 0;
+        for (int64_t i = tid; i < n * NQ; i += 256) {
+            const int64_t j = i / NQ;
+            const int d = 4 * (int)(i % NQ);
+            if (!placed(r + j)) continue;
+            const f4 x = key4(j, d), y = *reinterpret_cast<const f4 *>(V + j * a.ldv + d);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                tk = max(tk, __float_as_uint(x[u]) & 0x7FFFFFFFu);
+                tv = max(tv, __float_as_uint(y[u]) & 0x7FFFFFFFu);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            tk = max(tk, (uint32_t)__shfl_xor(tk, d));
+            tv = max(tv, (uint32_t)__shfl_xor(tv, d));
+        }
+        if (lane == 0) {
+            top[0][tid >> 6] = tk;
+            top[1][tid >> 6] = tv;
+        }
+        __syncthreads();
+        tk = max(max(top[0][0], top[0][1]), max(top[0][2], top[0][3]));
+        tv = max(max(top[1][0], top[1][1]), max(top[1][2], top[1][3]));
+        const bool fresh = row_of[0] >= 0;
+        const Scale sk = next_scale<FMT>(tk, old_k, fresh), sv = next_scale<FMT>(tv, old_v, fresh);
+        if (tid == 0) a.ks[at] = sk.s;
+        if (tid == 64) a.vs[at] = sv.s;
+        const bool bad_k = sk.s != sk.s, bad_v = sv.s != sv.s;
+        const float fk = ldexpf(1.0f, -sk.d), fv = ldexpf(1.0f, -sv.d);
+        uint8_t *kb = a.k + at * bt * D, *vb = a.v + at * bt * D;
+        // keys: unit u holds 16 dimensions of one token
+        for (int u = tid; u < bt * D / 16; u += 256) {
+            const int g = u & 3, rr = (u >> 2) & 3, c = (u >> 4) % C, t = (u >> 4) / C % 4, grp = u / D;
+            const int32_t j = row_of[16 * grp + 4 * t + rr];
+            u4 *to = reinterpret_cast<u4 *>(kb) + u;
+            u4 w = {0u, 0u, 0u, 0u};
+            if (j >= 0 && !bad_k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f4 x = key4(j, 64 * c + 16 * g + 4 * i);
+                    const float xs[4] = {x[0], x[1], x[2], x[3]};
+                    w[i] = F::pack(xs, sk.s, sk.inv);
+                }
+            } else if (j < 0 && !fresh) {
+                if (sk.d == 0) continue;
+                w = *to;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = F::shrink(w[i], fk);
+            }
+            *to = w;
+        }
+        // values: unit u holds 16 tokens at one dimension
+        for (int u = tid; u < bt * D / 16; u += 256) {
+            const int grp = u / D, d = u % D;
+            u4 *to = reinterpret_cast<u4 *>(vb) + u;
+            uint32_t fresh_bytes = 0;   // bit i: token i is new
+#pragma unroll
+            for (int i = 0; i < 16; ++i) fresh_bytes |= row_of[16 * grp + i] >= 0 ? 1u << i : 0u;
+            if (fresh_bytes == 0 && !fresh && sv.d == 0) continue;
+            u4 w = {0u, 0u, 0u, 0u};
+            if (!fresh && fresh_bytes != 0xFFFFu) {
+                w = *to;
+                if (sv.d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = F::shrink(w[i], fv);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(fresh_bytes >> (4 * i) & 15)) continue;
+                float x[4];
+                uint32_t keep = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int32_t j = row_of[16 * grp + 4 * i + b];
+                    x[b] = j >= 0 && !bad_v ? V[j * a.ldv + d] : 0.0f;
+                    if (j < 0) keep |= 0xFFu << (8 * b);
+                }
+                w[i] = (w[i] & keep) | (F::pack(x, sv.s, sv.inv) & ~keep);
+            }
+            *to = w;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- read
+// Workgroup (x, y): rows 16 x .. 16 x + 15 of KV head y; consecutive lanes
+// write consecutive floats.  A token's values lie 16 bytes apart, and the 16
+// rows, when they are one group of tokens, find them in the same lines.
+template <int FMT, int D>
+__global__ void __launch_bounds__(256)
+read_kernel(const uint8_t *__restrict__ k, const uint8_t *__restrict__ v, const float *__restrict__ ks,
+            const float *__restrict__ vs, const int32_t *__restrict__ slots, int64_t rows, int32_t heads,
+            int32_t n_blocks, int32_t shift, float *__restrict__ K, int64_t ldk, float *__restrict__ V, int64_t ldv)
+{
+    typedef Format<FMT> F;
+    constexpr int C = D / 64, NQ = D / 4;
+    const int head = blockIdx.y;
+    for (int i = threadIdx.x; i < 16 * NQ; i += 256) {
+        const int64_t r = (int64_t)blockIdx.x * 16 + i / NQ;
+        if (r >= rows) continue;
+        const int d = 4 * (i % NQ);
+        const int32_t slot = slots[r], b = slot >> shift;
+        f4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+        if (slot >= 0 && b < n_blocks) {
+            const int64_t at = (int64_t)b * heads + head;
+            const int o = slot & ((1 << shift) - 1), t = (o >> 2) & 3, rr = o & 3;
+            const int64_t base = (at << shift) * D + (int64_t)(o >> 4) * 16 * D;
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(
+                k + base + (((t * C + d / 64) * 4 + rr) * 4 + d % 64 / 16) * 16 + d % 16);
+            const float sk = ks[at], sv = vs[at];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                x[u] = F::value(w >> (8 * u) & 0xFF) * sk;
+                y[u] = F::value(v[base + (d + u) * 16 + (o & 15)]) * sv;
+            }
+        }
+        float *kr = K + r * ldk + head * D + d, *vr = V + r * ldv + head * D + d;
+        *reinterpret_cast<f4 *>(kr) = x;
+        *reinterpret_cast<f4 *>(vr) = y;
+    }
+}
+
+// Up to this many rows a plan's one workgroup also places them; more are
+// placed by a second launch over the whole device.
+constexpr int64_t kPlaceRows = 4096;
+// Up to this many rows every workgroup of an append looks at one row, above
+// at 16: a prompt's rows come in runs, and a run is the work of its first row.
+constexpr int64_t kSingleRows = 2048;
+
+template <int FMT, int D>
+void launch_append(const AppendArgs &a, bool rope, int rpw, hipStream_t stream)
+{
+    const dim3 grid((unsigned)((a.rows + rpw - 1) / rpw), (unsigned)(a.heads + (rope ? a.q_parts : 0)));
+    if (rope) hipLaunchKernelGGL((append_kernel<FMT, D, true>), grid, dim3(256), 0, stream, a, rpw);
+    else hipLaunchKernelGGL((append_kernel<FMT, D, false>), grid, dim3(256), 0, stream, a, rpw);
+}
+
+int append(aih_ctx *ctx, const aih_kv_cache *kv, AppendArgs a, bool rope)
+{
+    const int64_t wide = (int64_t)kv->n_kv_heads * kv->head_dim;
+    if (!a.K || !a.V || !a.slots || a.rows < 0 || a.ldk < wide || a.ldv < wide || a.ldk % 4 || a.ldv % 4 ||
+        !aih_kv::aligned16(a.K) || !aih_kv::aligned16(a.V))
+        return AIH_E_INVALID;
+    if (a.rows == 0) return AIH_OK;
+    if (a.rows > 0x7FFFFFFF) return AIH_E_LIMIT;
+    a.k = static_cast<uint8_t *>(kv->k);
+    a.v = static_cast<uint8_t *>(kv->v);
+    a.ks = kv->k_scale;
+    a.vs = kv->v_scale;
+    a.heads = kv->n_kv_heads;
+    a.n_blocks = kv->n_blocks;
+    a.shift = aih_kv::log2_of(kv->block_tokens);
+    a.q_parts = rope ? (int32_t)std::min<int64_t>(8, ((int64_t)a.q_heads * kv->head_dim + 1023) / 1024) : 0;
+    if (a.heads + a.q_parts > 65535) return AIH_E_LIMIT;
+    const int rpw = a.rows <= kSingleRows ? 1 : 16;
+    aih_kv::DeviceGuard guard(ctx->device);
+    AIH_TRY(guard.status);
+    const bool i8 = kv->format == AIH_KV_INT8;
+    switch (kv->head_dim) {
+    case 64: i8 ? launch_append<AIH_KV_INT8, 64>(a, rope, rpw, ctx->stream) : launch_append<AIH_KV_E4M3, 64>(a, rope, rpw, ctx->stream); break;
+    case 128: i8 ? launch_append<AIH_KV_INT8, 128>(a, rope, rpw, ctx->stream) : launch_append<AIH_KV_E4M3, 128>(a, rope, rpw, ctx->stream); break;
+    default: i8 ? launch_append<AIH_KV_INT8, 256>(a, rope, rpw, ctx->stream) : launch_append<AIH_KV_E4M3, 256>(a, rope, rpw, ctx->stream); break;
+    }
+    return aih_launch_status();
+}
+
+template <int FMT, int D>
+void launch_read(aih_ctx *ctx, const aih_kv_cache *kv, const int32_t *slots, int64_t rows, float *K, int64_t ldk,
+                 float *V, int64_t ldv)
+{
+    hipLaunchKernelGGL((read_kernel<FMT, D>), dim3((unsigned)((rows + 15) / 16), (unsigned)kv->n_kv_heads), dim3(256),
+                       0, ctx->stream, static_cast<const uint8_t *>(kv->k), static_cast<const uint8_t *>(kv->v),
+                       kv->k_scale, kv->v_scale, slots, rows, kv->n_kv_heads, kv->n_blocks,
+                       aih_kv::log2_of(kv->block_tokens), K, ldk, V, ldv);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t aih_kv_cache_bytes(const aih_kv_cache *kv)
+{
+    const int rc = aih_kv::check_shape(kv);
+    if (rc) return rc;
+    return (int64_t)kv->n_blocks * kv->block_tokens * kv->n_kv_heads * kv->head_dim;
+}
+
+int aih_kv_plan(aih_ctx *ctx, const int32_t *lens, const int32_t *n_new, int32_t n_seqs, int32_t *tables,
+                int32_t table_width, int32_t block_tokens, int32_t n_blocks, const int32_t *free_blocks,
+                const int32_t *n_free, int32_t *new_lens, int32_t *new_n_free, int32_t *starts, int32_t *slots,
+                int32_t *positions, int64_t rows, int32_t *refused)
+{
+    if (!ctx || !lens || !n_new || !tables || !free_blocks || !n_free || !new_lens || !new_n_free || !starts ||
+        !slots || !positions || !refused || n_seqs <= 0 || table_width <= 0 || n_blocks <= 0 || rows < 0)
+        return AIH_E_INVALID;
+    if (block_tokens != 16 && block_tokens != 32 && block_tokens != 64 && block_tokens != 128 && block_tokens != 256)
+        return AIH_E_UNSUPPORTED;
+    if (n_seqs > kMaxSeqs || rows > 0x7FFFFFFF || (int64_t)n_blocks * block_tokens > 0x7FFFFFFF ||
+        (int64_t)table_width * block_tokens > 0x7FFFFFFF)
+        return AIH_E_LIMIT;
+    aih_kv::DeviceGuard guard(ctx->device);
+    AIH_TRY(guard.status);
+    PlanArgs a{lens, n_new, tables, free_blocks, n_free, new_lens, new_n_free, starts, slots, positions, refused,
+               n_seqs, table_width, aih_kv::log2_of(block_tokens), n_blocks, (int32_t)rows};
+    const bool alone = rows <= kPlaceRows;
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, ctx->stream, a, alone ? 1 : 0);
+    if (!alone) {
+        const int rc = aih_launch_status();
+        if (rc) return rc;
+        hipLaunchKernelGGL(place_kernel, dim3((unsigned)std::min<int64_t>((rows + 255) / 256, 8192)), dim3(256), 0,
+                           ctx->stream, a);
+    }
+    return aih_launch_status();
+}
+
+int aih_kv_release(aih_ctx *ctx, int32_t *lens, int32_t n_seqs, int32_t *tables, int32_t table_width,
+                   int32_t block_tokens, int32_t n_blocks, const int32_t *done, int32_t *free_blocks, int32_t *n_free)
+{
+    if (!ctx || !lens || !tables || !free_blocks || !n_free || n_seqs <= 0 || table_width <= 0 || n_blocks <= 0)
+        return AIH_E_INVALID;
+    if (block_tokens != 16 && block_tokens != 32 && block_tokens != 64 && block_tokens != 128 && block_tokens != 256)
+        return AIH_E_UNSUPPORTED;
+    if (n_seqs > kMaxSeqs || (int64_t)n_blocks * block_tokens > 0x7FFFFFFF ||
+        (int64_t)table_width * block_tokens > 0x7FFFFFFF)
+        return AIH_E_LIMIT;
+    aih_kv::DeviceGuard guard(ctx->device);
+    AIH_TRY(guard.status);
+    hipLaunchKernelGGL(release_kernel, dim3(1), dim3(1024), 0, ctx->stream, lens, n_seqs, tables, table_width,
+                       aih_kv::log2_of(block_tokens), n_blocks, done, free_blocks, n_free);
+    return aih_launch_status();
+}
+
+int aih_kv_append(aih_ctx *ctx, const aih_kv_cache *kv, const float *K, int64_t ldk, const float *V, int64_t ldv,
+                  const int32_t *slots, int64_t rows)
+{
+    if (!ctx) return AIH_E_INVALID;
+    const int rc = aih_kv::check_cache(kv);
+    if (rc) return rc;
+    AppendArgs a{};
+    a.K = K;
+    a.V = V;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.slots = slots;
+    a.rows = rows;
+    return append(ctx, kv, a, false);
+}
+
+int aih_kv_append_rope(aih_ctx *ctx, const aih_kv_cache *kv, float *Q, int64_t ldq, int32_t n_heads, const float *K,
+                       int64_t ldk, const float *V, int64_t ldv, const int32_t *slots, const int32_t *positions,
+                       int64_t rows, const float *table, int32_t table_rows)
+{
+    if (!ctx) return AIH_E_INVALID;
+    const int rc = aih_kv::check_cache(kv);
+    if (rc) return rc;
+    if (!Q || !positions || !table || n_heads <= 0 || table_rows <= 0 || ldq < (int64_t)n_heads * kv->head_dim ||
+        ldq % 4 || !aih_kv::aligned16(Q) || !aih_kv::aligned16(table))
+        return AIH_E_INVALID;
+    AppendArgs a{};
+    a.K = K;
+    a.V = V;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.slots = slots;
+    a.rows = rows;
+    a.Q = Q;
+    a.ldq = ldq;
+    a.positions = positions;
+    a.table = table;
+    a.table_rows = table_rows;
+    a.q_heads = n_heads;
+    return append(ctx, kv, a, true);
+}
+
+int aih_kv_read(aih_ctx *ctx, const aih_kv_cache *kv, const int32_t *slots, int64_t rows, float *K, int64_t ldk,
+                float *V, int64_t ldv)
+{
+    if (!ctx) return AIH_E_INVALID;
+    const int rc = aih_kv::check_cache(kv);
+    if (rc) return rc;
+    const int64_t wide = (int64_t)kv->n_kv_heads * kv->head_dim;
+    if (!slots || !K || !V || rows < 0 || ldk < wide || ldv < wide || ldk % 4 || ldv % 4 || !aih_kv::aligned16(K) ||
+        !aih_kv::aligned16(V))
+        return AIH_E_INVALID;
+    if (rows == 0) return AIH_OK;
+    if (rows > 0x7FFFFFFF || kv->n_kv_heads > 65535) return AIH_E_LIMIT;
+    aih_kv::DeviceGuard guard(ctx->device);
+    AIH_TRY(guard.status);
+    const bool i8 = kv->format == AIH_KV_INT8;
+    switch (kv->head_dim) {
+    case 64: i8 ? launch_read<AIH_KV_INT8, 64>(ctx, kv, slots, rows, K, ldk, V, ldv) : launch_read<AIH_KV_E4M3, 64>(ctx, kv, slots, rows, K, ldk, V, ldv); break;
+    case 128: i8 ? launch_read<AIH_KV_INT8, 128>(ctx, kv, slots, rows, K, ldk, V, ldv) : launch_read<AIH_KV_E4M3, 128>(ctx, kv, slots, rows, K, ldk, V, ldv); break;
+    default: i8 ? launch_read<AIH_KV_INT8, 256>(ctx, kv, slots, rows, K, ldk, V, ldv) : launch_read<AIH_KV_E4M3, 256>(ctx, kv, slots, rows, K, ldk, V, ldv); break;
+    }
+    return aih_launch_status();
+}
+
+}  // extern "C"

@@ -510,6 +510,152 @@ int aih_attention_decode_qkv(aih_ctx *ctx, const float *QKV, float *Kc, float *V
                              const float *table, int32_t table_rows, int32_t max_len, float scale, float *scratch,
                              int64_t scratch_floats);
 
+/* ---- paged 8-bit KV cache ------------------------------------------------
+ *
+ * The keys and values of many requests in blocks of block_tokens tokens from
+ * one pool, one byte per value, with one fp32 scale per block and KV head for
+ * the keys and one for the values: a quarter of the memory and of the decode
+ * traffic of the fp32 cache, and no memory reserved for tokens that do not
+ * come.  The reference keeps one fp32 cache per conversation
+ * (InferenceEngine.cs:585-622); it has no counterpart to these operators.
+ *
+ * A code c of a block stands for c * scale:
+ *   AIH_KV_INT8  c a two's complement byte, -127..127
+ *   AIH_KV_E4M3  c a float of 1 sign, 4 exponent and 3 mantissa bits (OCP
+ *                FP8 E4M3), at most 448 in magnitude
+ * The scale follows the values as they come (a: the largest magnitude of the
+ * new values, Cmax: the largest code).  A block's first token (slot
+ * offset 0) starts it anew: all its codes are 0 and it has no scale.  The
+ * first a > 0 sets the scale: a / 127 rounded to fp32 (int8), or the smallest
+ * power of two s with a <= 448 s (e4m3); at least 2^-126.  A later
+ * a > Cmax * scale doubles the scale until a fits, and the codes already there
+ * are divided by the same power of two and rounded, so that however often
+ * it happens a code ends within one step of its value.  All codes are rounded to
+ * nearest, ties to even, from the exact quotient.  A value that is not
+ * finite makes its block's scale (of that head, keys or values) NaN, and with
+ * it everything the block stands for, until the block is started anew.
+ *
+ * Layout: block b of head h starts at byte (b * n_kv_heads + h) *
+ * block_tokens * head_dim of k and of v, its scales are k_scale and
+ * v_scale[b * n_kv_heads + h].  It holds its tokens in groups of 16, each as
+ * the 16-byte units that the matrix cores' lanes load.  In a group of keys,
+ * byte i of unit ((t * C + c) * 4 + r) * 4 + g is token 4t + r at
+ * dimension 64c + 16g + i (C = head_dim / 64); in a group of values byte i
+ * of unit d is token i at dimension d.  k and v: aih_kv_cache_bytes bytes
+ * each, 16-byte aligned.  A slot is block * block_tokens + offset. */
+#define AIH_KV_INT8 0
+#define AIH_KV_E4M3 1
+typedef struct aih_kv_cache {
+    int32_t format;        /* AIH_KV_INT8 or AIH_KV_E4M3                    */
+    int32_t n_kv_heads;
+    int32_t head_dim;      /* 64, 128 or 256                                */
+    int32_t block_tokens;  /* 16, 32, 64, 128 or 256                        */
+    int32_t n_blocks;      /* n_blocks * block_tokens < 2^31                */
+    int32_t reserved;      /* 0                                             */
+    void   *k, *v;
+    float  *k_scale, *v_scale;
+} aih_kv_cache;
+
+/* Bytes of the key codes (and of the value codes) of such a cache, or a
+ * negative status; the pointers are not looked at.  Needs no context and no
+ * device. */
+int64_t aih_kv_cache_bytes(const aih_kv_cache *kv);
+
+/* The bookkeeping of one step, on the device.  Request s holds lens[s] tokens
+ * in the blocks tables[s * table_width ..] and adds n_new[s].  The blocks it
+ * needs beyond those it has come off the end of the stack free_blocks[0 ..
+ * *n_free) (n_blocks ints of room), in request order, into its table; then
+ *   starts[s], s = 0..n_seqs   the first of its rows among the step's rows
+ *   new_lens[s]                lens[s] plus its rows
+ *   slots[r], positions[r]     for r < rows: where row r's token goes and its
+ *                              position in its request, -1 past the last row
+ *   *new_n_free                what is left on the stack
+ *   *refused                   the number of requests refused
+ * A request is refused as a whole, and gets no rows, when lens[s] or n_new[s]
+ * is negative, when the sum passes table_width * block_tokens, when the
+ * blocks needed by it and the requests before it pass *n_free (one that needs
+ * none is not held back by this), or when their rows pass `rows`; requests
+ * refused for one of the last two reasons count for those behind them.  new_lens
+ * may be lens and new_n_free n_free; where they are other arrays, a plan that
+ * is not carried out changes nothing but table entries past the requests'
+ * lengths.  A table entry outside [0, n_blocks) gives the slot -1.  n_seqs at
+ * most 4096 (AIH_E_LIMIT). */
+int aih_kv_plan(aih_ctx *ctx, const int32_t *lens, const int32_t *n_new, int32_t n_seqs, int32_t *tables,
+                int32_t table_width, int32_t block_tokens, int32_t n_blocks, const int32_t *free_blocks,
+                const int32_t *n_free, int32_t *new_lens, int32_t *new_n_free, int32_t *starts, int32_t *slots,
+                int32_t *positions, int64_t rows, int32_t *refused);
+
+/* Give the blocks of the requests with done[s] != 0 (all of them when done is
+ * NULL) back to the stack, in request and table order, and set their lens to
+ * 0 and those table entries to -1.  Entries outside [0, n_blocks), and blocks past
+ * the stack's n_blocks, are dropped.  n_seqs at most 4096. */
+int aih_kv_release(aih_ctx *ctx, int32_t *lens, int32_t n_seqs, int32_t *tables, int32_t table_width,
+                   int32_t block_tokens, int32_t n_blocks, const int32_t *done, int32_t *free_blocks, int32_t *n_free);
+
+/* Quantize key and value rows (row r at K + r * ldk and V + r * ldv,
+ * n_kv_heads * head_dim floats) into the cache at slots[r]; rows whose slot
+ * is outside the cache are skipped, whatever they hold.  The rows of one
+ * block have to follow one another (in any order of offsets; of two for the
+ * same slot the later one stays, and both count for the scale), as
+ * aih_kv_plan places them: a block that comes up again later in the same call
+ * ends with unspecified contents.  K, V 16-byte aligned, ldk and ldv
+ * multiples of 4. */
+int aih_kv_append(aih_ctx *ctx, const aih_kv_cache *kv, const float *K, int64_t ldk, const float *V, int64_t ldv,
+                  const int32_t *slots, int64_t rows);
+
+/* aih_kv_append with the rotation of aih_rope in the same launch: the
+ * n_heads query heads of row r of Q (ldq floats apart) in place and its keys on
+ * their way into the cache, both to positions[r]; the same results, bit for
+ * bit, as aih_rope and then aih_kv_append.  Rows whose position is outside
+ * [0, table_rows) are neither rotated nor stored.  Q, table 16-byte aligned, ldq
+ * a multiple of 4; Q, K and V may be parts of one projection's rows. */
+int aih_kv_append_rope(aih_ctx *ctx, const aih_kv_cache *kv, float *Q, int64_t ldq, int32_t n_heads, const float *K,
+                       int64_t ldk, const float *V, int64_t ldv, const int32_t *slots, const int32_t *positions,
+                       int64_t rows, const float *table, int32_t table_rows);
+
+/* The keys and values that the cache holds at slots[r], as fp32 rows
+ * (code * scale) of n_kv_heads * head_dim floats into K + r * ldk and
+ * V + r * ldv; zeros for a slot outside the cache. */
+int aih_kv_read(aih_ctx *ctx, const aih_kv_cache *kv, const int32_t *slots, int64_t rows, float *K, int64_t ldk,
+                float *V, int64_t ldv);
+
+/* What changes the scores of aih_kv_attention; zeros and NULLs change nothing. */
+typedef struct aih_kv_scores {
+    float          cap;      /* > 0: cap * tanh(score / cap)                       */
+    int32_t        window;   /* > 0: only the last `window` tokens, the own included */
+    const float   *slopes;   /* n_heads floats, or NULL: - slope * |distance|      */
+    const int32_t *prefix;   /* n_seqs ints, or NULL: the first prefix[s] tokens of
+                                request s are seen by all of its rows             */
+} aih_kv_scores;
+
+/* Grouped-query attention of a ragged batch over the cache.  Request s has
+ * the query rows starts[s] .. starts[s+1]-1 of Q, the last ones of the lens[s]
+ * tokens that the cache holds of it (its new tokens are appended first): row
+ * i of its n is at position p = lens[s] - n + i.  Head h attends to KV head
+ * h / (n_heads / n_kv_heads):
+ *   x_j = scale * (q . k_j),  x_j <- cap tanh(x_j / cap),  x_j <- x_j - slope_h |p - j|
+ *   o = sum_j softmax(x)_j v_j  over  p - window < j < max(p + 1, prefix[s]), 0 <= j < lens[s]
+ * A row that sees no token (a position before the first, blocks outside the
+ * cache: a table entry outside [0, n_blocks) hides its tokens) gives zeros; what
+ * hidden tokens hold has no effect.  Rows of O outside every request stay as
+ * they were.  starts, lens and the tables are read on the device, so that a
+ * captured step replays over growing requests; `rows` (of Q and O) bounds
+ * starts, and table_width * block_tokens bounds lens.  Products are formed on
+ * the fp16 matrix cores with q and the probabilities split in two (22 bits; the
+ * codes are exact in fp16), sums, scales and the softmax in fp32.  The work is
+ * split over keys where the rows alone would leave CUs idle, by the lengths
+ * found on the device; the parts are joined in a fixed order from `scratch`
+ * (aih_kv_attention_scratch_floats floats, 16-byte aligned, nothing in it has
+ * to be set; calls that overlap need one each), so a result depends on the
+ * arguments alone.  scale > 0; Q, O 16-byte aligned, ldq, ldo multiples of 4;
+ * n_seqs at most 4096, n_heads a multiple of n_kv_heads; scores may be NULL. */
+int64_t aih_kv_attention_scratch_floats(aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows,
+                                        int32_t n_seqs, int32_t table_width);
+int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64_t ldq, float *O, int64_t ldo,
+                     int64_t rows, int32_t n_heads, int32_t n_seqs, const int32_t *starts, const int32_t *lens,
+                     const int32_t *tables, int32_t table_width, float scale, const aih_kv_scores *scores,
+                     float *scratch, int64_t scratch_floats);
+
 /* Quantized embedding gather: Y[i,:] = dequantized row ids[i] of a [vocab,
  * dim] table of `type` blocks (ids from device memory; an id outside
  * [0, vocab) gives zeros).  Bit-exact to aih_dequantize (IEEE fp16 scales).

@@ -1,0 +1,279 @@
+"""aih_kv_attention against the plain implementation (kv_ref.py, 64 bits).
+
+Two bars.  Every row and head stays within the worst case of its own
+arithmetic (kv_ref.attention's `bound`).  The 2-norm over all rows is within
+BAR: rounding errors of random sign add like the root of their number, so that
+a score of 2 D <= 512 products with partial sums of a few units (unit normal
+rows, scale 1 / sqrt(D): |partial sum| <= 8, half a step 2^-22) is off by about
+sqrt(512 / 3) 2^-22 = 3e-6 at the very most and 5e-7 typically, and a weighted mean of
+values by that share of the values' spread: 4e-6 with the weights' 2^-21.
+Capped scores start from queries four times as large (four times the bar).
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv_ref as R
+from aihost_amd import _native as nat
+from gpu_util import upload
+
+pytestmark = pytest.mark.gpu
+
+I32 = np.int32
+BAR = 4e-6
+
+
+class Batch:
+    """A full random cache, tables over it and queries, on the device."""
+
+    def __init__(self, device, fmt, heads, kv, dim, block, lens, new, width=None, pad=0, behind=0, seed=0, spread=4.0,
+                 q_size=1.0):
+        rng = self.rng = np.random.default_rng(seed + dim + block + len(lens))
+        self.dev, self.heads, self.dim, self.pad = device, heads, dim, pad
+        need = [-(-l // block) for l in lens]
+        self.width = width or max(1, max(need))
+        self.ref = R.Cache(fmt, kv, dim, block, max(1, sum(need)) + 2)
+        self.ref.fill_random(rng, spread)
+        ids = rng.permutation(self.ref.n_blocks)
+        self.tables, at = np.full((len(lens), self.width), -1), 0
+        for s, b in enumerate(need):
+            self.tables[s, :b] = ids[at:at + b]
+            at += b
+        self.lens = list(lens)
+        self.starts = np.concatenate([[0], np.cumsum(new)])
+        self.rows = int(self.starts[-1]) + behind
+        self.q = (q_size * rng.standard_normal((self.rows, heads, dim))).astype(np.float32)
+        self.scale = float(np.float32(1 / np.sqrt(dim)))
+
+    def run(self, cap=0.0, window=0, slopes=None, prefix=None, out=None, times=1, graph=False):
+        L, h = nat.lib(), self.dev.handle
+        k, v = self.ref.packed()
+        bufs = [upload(self.dev, k), upload(self.dev, v)] + [upload(self.dev, s.astype(np.float32)) for s in self.ref.scales]
+        c = nat.KvCache(format=self.ref.fmt, n_kv_heads=self.ref.heads, head_dim=self.dim, block_tokens=self.ref.block,
+                        n_blocks=self.ref.n_blocks, k=bufs[0].get_pointer(), v=bufs[1].get_pointer(),
+                        k_scale=bufs[2].get_pointer(), v_scale=bufs[3].get_pointer())
+        wide = self.heads * self.dim
+        ld = wide + self.pad
+        q = np.full((self.rows, ld), np.nan, np.float32)
+        q[:, :wide] = self.q.reshape(self.rows, wide)
+        o = np.full((self.rows, ld), -7, np.float32)
+        up = [upload(self.dev, x) for x in (q, o, self.starts.astype(I32), np.asarray(self.lens, I32),
+                                            self.tables.astype(I32))]
+        opt = [upload(self.dev, np.asarray(slopes, np.float32)) if slopes is not None else None,
+               upload(self.dev, np.asarray(prefix, I32)) if prefix is not None else None]
+        sc = nat.KvScores(cap=cap, window=window, slopes=opt[0] and opt[0].get_pointer(),
+                          prefix=opt[1] and opt[1].get_pointer())
+        floats = nat.check_size(L.aih_kv_attention_scratch_floats(h, ctypes.byref(c), self.heads, self.rows,
+                                                                  len(self.lens), self.width), "scratch")
+        sb = self.dev.create_buffer(max(16, 4 * floats))
+        sb.write(np.full(max(4, floats), np.nan, np.float32))     # nothing in it has to be set
+        for _ in range(times):
+            nat.check(L.aih_kv_attention(h, ctypes.byref(c), up[0].get_pointer(), ld, up[1].get_pointer(), ld, self.rows,
+                                         self.heads, len(self.lens), up[2].get_pointer(), up[3].get_pointer(),
+                                         up[4].get_pointer(), self.width, self.scale, ctypes.byref(sc),
+                                         sb.get_pointer(), floats), "aih_kv_attention")
+        self.dev.synchronize()
+        got = up[1].read_range(0, self.rows * ld, np.float32).reshape(self.rows, ld)
+        for b in bufs + up + [sb] + [x for x in opt if x]:
+            b.dispose()
+        assert np.all(got[:, wide:] == -7)
+        return got[:, :wide].reshape(self.rows, self.heads, self.dim)
+
+    def check(self, bar=BAR, **kw):
+        got = self.run(**kw)
+        want, bound = R.attention(self.ref, self.q, self.starts, self.lens, self.tables, self.scale, **kw)
+        n = int(self.starts[-1])
+        assert np.all(got[n:] == -7)            # rows behind the last request stay as they were
+        got, want, bound = got[:n], want[:n], bound[:n]
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        ok = ~np.isnan(want)
+        err = np.where(ok, np.abs(got - want), 0).max(-1)
+        assert np.all((err <= bound) | ~ok.all(-1)), "row, head %s: %.3g over %.3g" % (
+            np.unravel_index(np.argmax(err - bound), err.shape), err.max(), bound.max())
+        nrm = np.linalg.norm((got - want)[ok]) / max(np.linalg.norm(want[ok]), 1e-30)
+        assert nrm <= bar, nrm
+        return got
+
+
+FORMATS = [R.INT8, R.E4M3]
+
+
+def within(got, want, bound):
+    return bool(np.all(np.abs(got - want).max(-1) <= bound))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,block", [(8, 2, 16), (3, 3, 32), (5, 1, 64), (20, 1, 16), (6, 2, 256)])
+def test_single_tokens(device, fmt, dim, heads, kv, block):
+    """One token each, lengths from one to several parts, an empty request and padding between them."""
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 0, 255, 257, 700, 1030]
+    new = [1, 1, 1, 1, 1, 1, 1, 1, 0, 1, 1, 1, 1]
+    Batch(device, fmt, heads, kv, dim, block, lens, new, pad=4, behind=3).check()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,block,lens,new", [
+    (32, 8, 128, 16, [513], [1]), (32, 8, 128, 32, [5000], [1]), (8, 8, 64, 16, [2100, 33], [1, 1]),
+    (16, 8, 256, 64, [1500], [1]), (4, 4, 128, 16, [4096, 64, 1], [1, 1, 1])])
+def test_long_single_tokens(device, fmt, heads, kv, dim, block, lens, new):
+    Batch(device, fmt, heads, kv, dim, block, lens, new).check()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,block,lens,new", [
+    (8, 2, 128, 16, [4, 20, 300], [4, 4, 4]), (4, 4, 64, 32, [7, 130, 1025], [7, 2, 5]),
+    (10, 2, 128, 16, [40, 90], [3, 12]), (2, 1, 256, 16, [33, 90], [9, 1])])
+def test_a_few_tokens(device, fmt, heads, kv, dim, block, lens, new):
+    Batch(device, fmt, heads, kv, dim, block, lens, new).check()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,block,lens,new", [
+    (8, 2, 128, 16, [200], [200]), (4, 1, 128, 32, [1, 33, 65, 190, 0, 300], [1, 33, 65, 190, 0, 130]),
+    (3, 3, 64, 16, [257, 129], [257, 100]), (5, 1, 64, 64, [140], [140]), (4, 2, 256, 16, [150, 70], [150, 20]),
+    (8, 8, 128, 16, [130], [130]), (4, 1, 128, 64, [2500], [70]), (32, 1, 64, 16, [60], [60])])
+def test_prompts(device, fmt, heads, kv, dim, block, lens, new):
+    Batch(device, fmt, heads, kv, dim, block, lens, new, pad=8, behind=2).check()
+
+
+SCORES = [dict(cap=30.0), dict(cap=2.0), dict(window=1), dict(window=17), dict(window=64, cap=50.0), dict(slopes=True),
+          dict(slopes=True, cap=20.0, window=90), dict(prefix=[0, 20, 150]), dict(prefix=[300, 500, 5], window=40),
+          dict(prefix=[64, 1, 33], slopes=True, cap=10.0)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 3, 30], [200, 25, 160]])
+@pytest.mark.parametrize("scores", SCORES, ids=[str(i) for i in range(len(SCORES))])
+def test_scores(device, fmt, dim, new, scores):
+    scores = dict(scores)
+    if scores.get("slopes"):
+        scores["slopes"] = [2.0 ** -(1 + h) for h in range(4)]
+    cap = "cap" in scores
+    Batch(device, fmt, 4, 2, dim, 16, [300, 25, 160], new, q_size=4.0 if cap else 1.0).check(
+        bar=4 * BAR if cap else BAR, **scores)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [6, 2], [100, 90]])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_blocks_outside_the_cache(device, fmt, new):
+    """A table entry outside the pool hides its tokens; a row that sees none gives zeros."""
+    b = Batch(device, fmt, 4, 2, 128, 16, [330, 100], new)
+    b.tables[0, [0, 3, 20]] = [-1, b.ref.n_blocks, 2 ** 31 - 1]
+    b.tables[1, :] = -2 ** 31
+    got = b.check()
+    assert np.all(got[b.starts[1]:b.starts[2]] == 0)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [6, 2], [100, 90]])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_lengths_that_do_not_fit(device, fmt, new):
+    """More rows than tokens (rows before the first token see nothing), a negative length, a length past the table."""
+    b = Batch(device, fmt, 4, 2, 128, 16, [200, 96], new)
+    b.lens[0] = 0 if new[0] == 1 else new[0] - 3
+    want_zero = 1 if new[0] == 1 else 3
+    if new[0] == 1:
+        b.lens[0] = -5
+    got = b.run()
+    assert np.all(got[:want_zero] == 0)
+    b.lens[0] = max(b.lens[0], 0)
+    want, bound = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale)
+    assert within(got, want, bound)
+    b.lens = [200, 10 ** 9]
+    got = b.run()
+    b.lens = [200, b.width * 16]
+    want, bound = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale)
+    assert within(got, want, bound)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [6, 2], [100, 90]])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_what_hidden_tokens_hold_has_no_effect(device, fmt, new):
+    """Past the length, before the window, in another request's rows: NaN scales and values of 1e30."""
+    b = Batch(device, fmt, 4, 2, 128, 16, [200, 100], new)
+    plain = b.run(window=50)
+    seen = set()
+    for s in (0, 1):
+        low = max(0, b.lens[s] - new[s] - 49)
+        seen |= {int(b.tables[s, x // 16]) for x in range(low, b.lens[s])}
+    hidden = [x for x in range(b.ref.n_blocks) if x not in seen]
+    assert len(hidden) > 2
+    before_all = b.ref.scales.copy()
+    b.ref.scales[:, hidden[::2]] = np.nan
+    b.ref.scales[:, hidden[1::2]] = 1e30
+    np.testing.assert_array_equal(b.run(window=50), plain)
+    b.ref.scales = before_all
+    # a later token's block: rows before it are as exact as without it
+    n = new[0]
+    if n >= 100:
+        for bad in (np.nan, 1e30, 1e-30):
+            last = int(b.tables[0, 199 // 16])
+            b.ref.scales[:, last] = bad
+            got, (want, bound) = b.run(), R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale)
+            before = 192 - (200 - n)
+            fine = np.abs(got - want)[:before].max(-1) <= bound[:before]
+            assert fine.all(), (bad, fine.sum())
+            assert np.isnan(got[before:n]).all() == np.isnan(bad)
+
+
+@pytest.mark.parametrize("new", [[1], [5], [120]])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_scales_far_apart(device, fmt, new):
+    """Blocks of zeros (no scale), value scales from 2^-120 to 2^100, key scales from tiny to large."""
+    b = Batch(device, fmt, 4, 2, 128, 16, [400], new)
+    t = b.tables[0]
+    for values in ([0.0] * 5, [2.0 ** -120, 1.0, 0.0, 2.0 ** -60, 2.0 ** -10], [2.0 ** 100, 1.0, 0.0, 2.0 ** 60, 2.0 ** -20]):
+        for i, f in enumerate(values):
+            b.ref.scales[1, t[i::5]] = np.float32(f)
+            if f == 0:
+                b.ref.codes[1, t[i::5]] = 0
+        b.ref.scales[0, t[3]] = 0
+        b.ref.codes[0, t[3]] = 0
+        got = b.run()
+        want, bound = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale)
+        assert within(got, want, bound)
+    b.ref.scales[1, t[:25]] = np.float32(2.0 ** -126)     # all of them at the floor
+    b.ref.codes[1, t[:25]] = b.ref.codes[1, t[1]]
+    got = b.run()
+    want, bound = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale)
+    # values of 2^-119: an output is a multiple of 2^-149
+    assert within(got, want, bound + 2.0 ** -148)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [4, 3], [64, 70]])
+def test_queries_that_are_not_finite(device, new):
+    """A query with NaN or an infinity makes its own row NaN and no other."""
+    b = Batch(device, R.INT8, 4, 2, 64, 16, [90, 100], new)
+    plain = b.run()
+    b.q[0, 1, 5], b.q[b.starts[1], 2, 63] = np.nan, np.inf
+    got = b.run()
+    bad = np.zeros(got.shape[:2], bool)
+    bad[0, 1] = bad[b.starts[1], 2] = True
+    assert np.isnan(got[bad]).all()
+    np.testing.assert_array_equal(got[~bad], plain[~bad])
+    b.q[0, 1] = 0                                      # a zero query weighs all alike
+    b.q[b.starts[1], 2] = 1e30 * np.sign(b.q[b.starts[1], 2])      # a huge one picks one key
+    b.q[b.starts[1], 2, 63] = 1e30
+    got = b.run()
+    assert np.isfinite(got).all()
+
+
+def test_same_twice_and_over_many_requests(device):
+    """The same bits again; 900 requests of one token (several scan steps of 64)."""
+    lens = [1 + (7 * s) % 150 for s in range(900)]
+    b = Batch(device, R.INT8, 4, 2, 64, 16, lens, [1] * 900)
+    one = b.check()
+    np.testing.assert_array_equal(b.run(times=3), one)
+
+
+def test_shape_of_the_batch_does_not_change_a_short_row(device):
+    """Requests that are not split give the same bits alone and in a batch."""
+    b = Batch(device, R.E4M3, 8, 2, 128, 16, [100, 250, 3], [1, 1, 1])
+    both = b.run()
+    for s in range(3):
+        one = Batch.__new__(Batch)
+        one.__dict__.update(b.__dict__)
+        one.lens, one.tables, one.starts, one.rows, one.q = [b.lens[s]], b.tables[s:s + 1], np.array([0, 1]), 1, b.q[s:s + 1]
+        np.testing.assert_array_equal(one.run()[0], both[s])
