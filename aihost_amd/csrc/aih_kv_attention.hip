@@ -387,13 +387,19 @@ struct Lane {
     bool none;      // the group is not there
 };
 
-// Scores of a tile to split weights, and the state's normalizer, sum and
-// accumulator brought up to it.  s: the lane's 16 products of query c with keys
-// key0 + 0..15 (key0 = 64 tile + 16 g); f: the factor that makes them scores,
-// times log2 e unless MOD.  HIDE: some key of the tile is not seen by some query.
-template <int D, bool MOD, bool HIDE>
-__device__ __forceinline__ void softmax_tile(const Args &a, const Col &c, const Lane &ln, int32_t key0, float f,
-                                             f4 *s, State<D> &st, h8 *ph, h8 *pl)
+// What makes weights of a lane's products of one tile: p = 2^(f s + add), the
+// weight p vs, and the sum of the p times 2^-e into the state's.
+struct Weights {
+    float f, add, vs, e;
+};
+
+// The scores of a tile, and the state's normalizer and accumulator brought up to
+// them.  s: the lane's 16 products of query c with keys key0 + 0..15 (key0 = 64
+// tile + 16 g); f: the factor that makes them scores, times log2 e unless MOD.
+// hide (the same in all lanes): some key of the tile is not seen by some query.
+template <int D, bool MOD>
+__device__ __forceinline__ Weights score_tile(const Args &a, const Col &c, const Lane &ln, int32_t key0, float f,
+                                              bool hide, f4 *s, State<D> &st)
 {
     if constexpr (MOD) {
         float top = 0.f;
@@ -427,7 +433,7 @@ __device__ __forceinline__ void softmax_tile(const Args &a, const Col &c, const 
         f = 1.0f;
     }
     bool some = true;   // the query sees a key of this lane's group
-    if constexpr (HIDE) {
+    if (hide) {
         const int32_t lo = c.lo - key0, hi = ln.none ? -1 : c.hi - key0;
         some = lo < 16 && hi > 0;
 #pragma unroll
@@ -448,7 +454,7 @@ __device__ __forceinline__ void softmax_tile(const Args &a, const Col &c, const 
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
-    if constexpr (!MOD && !HIDE) {
+    if constexpr (!MOD) {
         // beyond 2^20 the rounding of a score is no longer small beside 1: the normalizer and the exponents below have to
         // come from the same rounded scores
         if (__any(mx * f > 0x1p20f)) {
@@ -465,28 +471,28 @@ __device__ __forceinline__ void softmax_tile(const Args &a, const Col &c, const 
         st.times(back);
         st.m = m;
     }
-    const float add = e - (m == -INFINITY ? 0.f : m);
-    float sum = 0.f;
+    return Weights{f, e - (m == -INFINITY ? 0.f : m), vs, e};
+}
+
+// The weights of keys 8 m + 0..7 of the lane's group, split; the sum of their p is added to `sum`.
+__device__ __forceinline__ void weigh(const Weights &w, bool hide, int m, const f4 *s, float &sum, h8 &ph, h8 &pl)
+{
+    uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = 2 * h + i / 2, u = 2 * (i % 2);
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][u], f, add)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][u + 1], f, add));
-            sum += p0;
-            sum += p1;
-            float w0 = p0 * vs, w1 = p1 * vs;
-            if constexpr (HIDE) {   // a hidden key's block may have no number for a scale
-                w0 = s[t][u] == -INFINITY ? 0.f : w0;
-                w1 = s[t][u + 1] == -INFINITY ? 0.f : w1;
-            }
-            split2(w0, w1, hi[i], lo[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float s0 = s[2 * m + i / 2][2 * (i % 2)], s1 = s[2 * m + i / 2][2 * (i % 2) + 1];
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s0, w.f, w.add)), p1 = __builtin_amdgcn_exp2f(fmaf(s1, w.f, w.add));
+        sum += p0;
+        sum += p1;
+        float w0 = p0 * w.vs, w1 = p1 * w.vs;
+        if (hide) {   // a hidden key's block may have no number for a scale
+            w0 = s0 == -INFINITY ? 0.f : w0;
+            w1 = s1 == -INFINITY ? 0.f : w1;
         }
-        ph[h] = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
-        pl[h] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
+        split2(w0, w1, hi[i], lo[i]);
     }
-    st.l += ldexpf(sum, -(int)e);
+    ph = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
+    pl = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
 }
 
 // ---------------------------------------------------------------- few rows: 16 at a time
@@ -553,19 +559,21 @@ few_kernel(Args a, int32_t heads)
                     s[q] = mfma(x, ql[k][m], s[q]);
                 }
         }
-        h8 ph[2], pl[2];
-        const int32_t key0 = t * 64 + 16 * g;
         const bool hide = t * 64 < see_lo || (int64_t)t * 64 + 64 > see_hi || __any(ln.none);
-        if (hide) softmax_tile<D, MOD, true>(a, col, ln, key0, undo * ln.ks, s, st, ph, pl);
-        else softmax_tile<D, MOD, false>(a, col, ln, key0, undo * ln.ks, s, st, ph, pl);
+        const Weights wt = score_tile<D, MOD>(a, col, ln, t * 64 + 16 * g, undo * ln.ks, hide, s, st);
+        float sum = 0.f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int m = 0; m < 2; ++m) {
+            h8 ph, pl;
+            weigh(wt, hide, m, s, sum, ph, pl);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
+            for (int d = 0; d < DT; ++d) {
                 const h8 x = to_half<FMT>(vr[d][2 * m], vr[d][2 * m + 1]);
-                st.o[d] = mfma(x, ph[m], st.o[d]);
-                st.o[d] = mfma(x, pl[m], st.o[d]);
+                st.o[d] = mfma(x, ph, st.o[d]);
+                st.o[d] = mfma(x, pl, st.o[d]);
             }
+        }
+        st.l += ldexpf(sum, -(int)wt.e);
     }
     // join the waves
     const float l = over4_sum(st.l);
@@ -604,6 +612,168 @@ few_kernel(Args a, int32_t heads)
             for (int u = 0; u < 4; ++u) x[u] += times2(y[u], ms[i][row] - m);
         }
         *reinterpret_cast<f4 *>(to + d) = x * div;
+    }
+}
+
+// ---------------------------------------------------------------- many rows: 128 at a time
+constexpr int kPromptRows = 128;
+
+// Workgroup (head fastest): a part of one tile of 128 rows, 32 to a wave.  The
+// codes of a key tile are converted to fp16 once, into LDS, in the order in
+// which the lanes read them (unit by unit, so every LDS access is 1 KB in a row),
+// and every fragment read feeds the four products of two column tiles and
+// two halves.  Two images: while a tile is multiplied, the next one, loaded a tile
+// ago, is converted, and the one after it is loaded.  One barrier per tile.
+template <int FMT, int D, bool MOD>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+prompt_kernel(Args a, int32_t heads)
+{
+    constexpr int C = D / 64, DT = D / 16;
+    __shared__ h8 image[2][2][4 * C * 2 * 64];   // [buffer][keys, values][(unit row, half)][lane]
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int32_t kvh = blockIdx.x % heads;
+    const Item it = find_item<kPromptRows>(a, blockIdx.x / heads, heads, false);
+    if (!it.ok) return;
+    const Range all = tile_keys<kPromptRows>(a, it), mine = part_of(all, it.split, it.n_split);
+
+    Col col[2];
+    h8 qh[2][C][2], ql[2][C][2];
+    float undo[2];
+    int32_t see_lo[2], see_hi[2];               // what every query of a column tile sees
+    int32_t any_lo = 0x7FFFFFFF, any_hi = 0;    // and any of the wave's
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        col[n] = column(a, it, kvh, (int64_t)it.tile * kPromptRows + 32 * w + 16 * n + c);
+        undo[n] = load_q<D>(a, col[n], g, qh[n], ql[n]) * a.scale * (MOD ? 1.0f : kLog2e);
+        const bool is = col[n].token >= 0;
+        see_lo[n] = is ? col[n].lo : 0;
+        see_hi[n] = is ? col[n].hi : 0x7FFFFFFF;
+        if (is) {
+            any_lo = min(any_lo, col[n].lo);
+            any_hi = max(any_hi, col[n].hi);
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            see_lo[n] = max(see_lo[n], __shfl_xor(see_lo[n], d));
+            see_hi[n] = min(see_hi[n], __shfl_xor(see_hi[n], d));
+        }
+        see_lo[n] = __builtin_amdgcn_readfirstlane(see_lo[n]);
+        see_hi[n] = __builtin_amdgcn_readfirstlane(see_hi[n]);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        any_lo = min(any_lo, __shfl_xor(any_lo, d));
+        any_hi = max(any_hi, __shfl_xor(any_hi, d));
+    }
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+
+    State<D> st[2];
+    st[0].init();
+    st[1].init();
+    Groups gr{kNone, 0.f, 0.f};
+    u4 kr[C], vr[C];
+    // loads tile t (this thread's units of it) and returns what its lane needs of it
+    auto load = [&](int32_t t) {
+        Lane ln{0.f, 0.f, true};
+        if (t >= mine.hi) return ln;
+        const int in = (t - mine.lo) & 15;
+        if (in == 0) gr = load_groups(a, it.seq, it.q.len, kvh, heads, t);
+        const uint32_t at_k = __shfl(gr.at, 4 * in + (c >> 2)), at_v = __shfl(gr.at, 4 * in + g);
+        ln.ks = __shfl(gr.ks, 4 * in + g);
+        ln.vs = __shfl(gr.vs, 4 * in + g);
+        ln.none = at_v == kNone;
+        const uint8_t *kp = a.k + (size_t)(at_k == kNone ? 0 : at_k) * (16 * D) + ((c & 3) * 4 + g) * 16 + w * 256;
+        const uint8_t *vp = a.v + (size_t)(at_v == kNone ? 0 : at_v) * (16 * D) + c * 16 + w * 256;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            kr[i] = *reinterpret_cast<const u4 *>(kp + i * 1024);
+            vr[i] = *reinterpret_cast<const u4 *>(vp + i * 1024);
+        }
+        return ln;
+    };
+    auto convert = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                image[b][0][((w + 4 * i) * 2 + m) * 64 + lane] = to_half<FMT>(kr[i][2 * m], kr[i][2 * m + 1]);
+                image[b][1][((w + 4 * i) * 2 + m) * 64 + lane] = to_half<FMT>(vr[i][2 * m], vr[i][2 * m + 1]);
+            }
+    };
+    Lane ln = load(mine.lo), next{};
+    if (mine.lo < mine.hi) convert(0);
+    next = load(mine.lo + 1);
+    __syncthreads();
+    for (int32_t t = mine.lo; t < mine.hi; ++t) {
+        const int b = (t - mine.lo) & 1;
+        const bool work = t * 64 < any_hi && (int64_t)t * 64 + 64 > any_lo;
+        f4 s[2][4];
+        Weights wt[2];
+        bool hide[2] = {false, false};
+        if (work) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                s[0][q] = s[1][q] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < C; ++k)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const h8 x = image[b][0][((q * C + k) * 2 + m) * 64 + lane];
+                        s[0][q] = mfma(x, qh[0][k][m], s[0][q]);
+                        s[1][q] = mfma(x, qh[1][k][m], s[1][q]);
+                        s[0][q] = mfma(x, ql[0][k][m], s[0][q]);
+                        s[1][q] = mfma(x, ql[1][k][m], s[1][q]);
+                    }
+            }
+            const bool none = __any(ln.none);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                hide[n] = none || t * 64 < see_lo[n] || (int64_t)t * 64 + 64 > see_hi[n];
+                wt[n] = score_tile<D, MOD>(a, col[n], ln, t * 64 + 16 * g, undo[n] * ln.ks, hide[n], s[n], st[n]);
+            }
+        }
+        if (t + 1 < mine.hi) convert(b ^ 1);
+        ln = next;
+        next = load(t + 2);
+        if (work) {
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                h8 ph[2], pl[2];
+                weigh(wt[0], hide[0], m, s[0], sum[0], ph[0], pl[0]);
+                weigh(wt[1], hide[1], m, s[1], sum[1], ph[1], pl[1]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const h8 x = image[b][1][(d * 2 + m) * 64 + lane];
+                    st[0].o[d] = mfma(x, ph[0], st[0].o[d]);
+                    st[1].o[d] = mfma(x, ph[1], st[1].o[d]);
+                    st[0].o[d] = mfma(x, pl[0], st[0].o[d]);
+                    st[1].o[d] = mfma(x, pl[1], st[1].o[d]);
+                }
+            }
+            st[0].l += ldexpf(sum[0], -(int)wt[0].e);
+            st[1].l += ldexpf(sum[1], -(int)wt[1].e);
+        }
+        __syncthreads();
+    }
+    const bool whole = it.n_split == 1;
+    const int32_t part = (it.part + it.split) * heads + kvh;
+    if (!whole && part >= a.n_part) return;   // never: the scratch is sized for every part
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const float sum = over4_sum(st[n].l);
+        if (col[n].token < 0) continue;
+        const int64_t row = (int64_t)part * kPromptRows + 32 * w + 16 * n + c;
+        float *to = whole ? a.O + (int64_t)col[n].token * a.ldo + col[n].head * D : a.part + row * D;
+        if (!whole && g == 0) {
+            a.part_ml[row * 2] = st[n].m;
+            a.part_ml[row * 2 + 1] = sum;
+        }
+        const float div = !whole ? 1.0f : sum != 0.f ? 0x1p-15f / sum : 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f4 *>(to + 16 * d + 4 * g) = st[n].o[d] * div;
     }
 }
 
@@ -662,9 +832,10 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
 {
     const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256, heads = kv->n_kv_heads, group = n_heads / heads;
     Plan p{};
-    p.rows = 16;
+    const bool few = rows * group <= 32 * (int64_t)n_seqs;
+    p.rows = few ? 16 : kPromptRows;
     p.least = 4;
-    p.target = 4 * cus;
+    p.target = (few ? 4 : 2) * cus;
     const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
     p.tiles = std::min<int64_t>(n_seqs, rows) + rows * group / p.rows;   // sum of ceil(n_s group / R) over the n_s > 0
     const int64_t most_split = (most_keys + p.least - 1) / p.least;
@@ -682,11 +853,15 @@ int64_t ml_floats(const Plan &p) { return (p.parts * p.rows * 2 + kAlign - 1) / 
 template <int FMT, int D, bool MOD>
 int launch(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
 {
-    hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), dim3((unsigned)(p.items * heads)), dim3(256), 0, ctx->stream, a, heads);
+    const bool few = p.rows == 16;
+    const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.tiles * heads)), block(256);
+    if (few) hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
+    else hipLaunchKernelGGL((prompt_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
     if (p.parts) {
         const int rc = aih_launch_status();
         if (rc) return rc;
-        hipLaunchKernelGGL((join_kernel<D, 16>), dim3((unsigned)(p.tiles * heads)), dim3(256), 0, ctx->stream, a, heads);
+        if (few) hipLaunchKernelGGL((join_kernel<D, 16>), join, block, 0, ctx->stream, a, heads);
+        else hipLaunchKernelGGL((join_kernel<D, kPromptRows>), join, block, 0, ctx->stream, a, heads);
     }
     return aih_launch_status();
 }
