@@ -103,67 +103,102 @@ struct Item {
     bool ok;
 };
 
-template <typename T>
-__device__ __forceinline__ T wave_add(T v)
+// Sum and inclusive scan over the 64 lanes on the DPP path (a shuffle goes
+// through LDS, ten times the latency): within rows of 16, then row 0 into row 1
+// and 2 into 3 (row_bcast:15), then rows 0, 1 into 2, 3 (row_bcast:31).
+__device__ __forceinline__ float wave_add(float v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x111, 0xF, 0xF, true);   // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x143, 0xC, 0xF, false);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ int32_t wave_scan(int32_t v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
+}
+
+// A lane's request: its row tiles and the key tiles of the longest of them.
+struct Load {
+    Seq q;
+    int32_t tiles, keys;
+};
+
+template <int R>
+__device__ __forceinline__ Load load_of(const Args &a, int s)
+{
+    Load l{{0, 0, 0}, 0, 0};
+    if (s < a.n_seqs) {
+        l.q = seq_of(a, s);
+        l.tiles = row_tiles<R>(a, l.q);
+        l.keys = max(key_tiles(a, l.q), 0);
+    }
+    return l;
 }
 
 // Item `idx` of one KV head: parts are numbered request by request, tile by
 // tile (the last, longest one first), split by split; with `joined`, tiles
-// instead.  Part length: the whole work over the wanted workgroups, so that
-// all parts are about as long whatever the requests' lengths.  Every wave of
-// the launch runs this with all lanes.
+// instead.  The longest part: the whole work over the wanted workgroups, so that
+// all parts are about as long whatever the requests' lengths; longer where
+// rounding up would make a few parts more than that number, which would run
+// alone after the others.  Every wave of the launch runs this with all lanes.
+// (The sums are floats: the same in every wave, and they only weigh the parts.)
 template <int R>
 __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t heads, bool joined)
 {
     const int lane = threadIdx.x & 63;
-    int64_t work = 0;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-        const int s = base + lane;
-        if (s < a.n_seqs) {
-            const Seq q = seq_of(a, s);
-            work += (int64_t)row_tiles<R>(a, q) * max(key_tiles(a, q), 0);
+    const Load first = load_of<R>(a, lane);
+    int32_t len = 1 << 30;   // nothing is split
+    if (a.n_part) {
+        float work = (float)first.tiles * (float)first.keys, tiles_all = (float)first.tiles;
+        for (int base = 64; base < a.n_seqs; base += 64) {
+            const Load l = load_of<R>(a, base + lane);
+            work += (float)l.tiles * (float)l.keys;
+            tiles_all += (float)l.tiles;
         }
-    }
-    work = wave_add(work) * heads;
-    const int32_t len = (int32_t)max<int64_t>(a.least, (work + a.target - 1) / a.target);
-    int32_t before = 0, parts = 0;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-        const int s = base + lane;
-        Seq q{0, 0, 0};
-        int32_t tiles = 0, n_split = 1;
-        if (s < a.n_seqs) {
-            q = seq_of(a, s);
-            tiles = row_tiles<R>(a, q);
-            n_split = max(1, (key_tiles(a, q) + len - 1) / len);
-        }
-        const int32_t own = joined ? tiles : tiles * n_split;
-        int32_t upto = own, part_upto = n_split > 1 ? tiles * n_split : 0;
-        const int32_t part_own = part_upto;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int32_t o = __shfl_up(upto, d), p = __shfl_up(part_upto, d);
-            if (lane >= d) {
-                upto += o;
-                part_upto += p;
+        const float want = (float)a.target / (float)heads;
+        len = max(a.least, (int32_t)ceilf(wave_add(work) / want));
+        if (wave_add(tiles_all) < want) {
+            for (int i = 0; i < 4; ++i) {
+                float n = (float)first.tiles * (float)((first.keys + len - 1) / len);
+                for (int base = 64; base < a.n_seqs; base += 64) {
+                    const Load l = load_of<R>(a, base + lane);
+                    n += (float)l.tiles * (float)((l.keys + len - 1) / len);
+                }
+                n = wave_add(n);
+                if (n <= want) break;
+                len = max(len + 1, (int32_t)((float)len * n / want));
             }
         }
+    }
+    int32_t before = 0, parts = 0;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const Load l = base ? load_of<R>(a, base + lane) : first;
+        const int32_t n_split = max(1, (l.keys + len - 1) / len);
+        const int32_t own = joined ? l.tiles : l.tiles * n_split, part_own = n_split > 1 ? l.tiles * n_split : 0;
+        const int32_t upto = wave_scan(own), part_upto = wave_scan(part_own);
         const unsigned long long past = __ballot(before + upto > idx);
         if (past) {
-            const int l = __builtin_ctzll(past);
+            const int at = __builtin_ctzll(past);
             Item it;
-            const int32_t k = idx - (before + __builtin_amdgcn_readlane(upto - own, l));
-            it.n_split = __builtin_amdgcn_readlane(n_split, l);
-            const int32_t nt = __builtin_amdgcn_readlane(tiles, l);
+            const int32_t k = idx - (before + __builtin_amdgcn_readlane(upto - own, at));
+            it.n_split = __builtin_amdgcn_readlane(n_split, at);
+            const int32_t nt = __builtin_amdgcn_readlane(l.tiles, at);
             it.tile = joined ? k : nt - 1 - k / it.n_split;
             it.split = joined ? 0 : k % it.n_split;
-            it.seq = base + l;
-            it.part = parts + __builtin_amdgcn_readlane(part_upto - part_own, l) + it.tile * it.n_split;
-            it.q = Seq{__builtin_amdgcn_readlane(q.start, l), __builtin_amdgcn_readlane(q.n, l),
-                       __builtin_amdgcn_readlane(q.len, l)};
+            it.seq = base + at;
+            it.part = parts + __builtin_amdgcn_readlane(part_upto - part_own, at) + it.tile * it.n_split;
+            it.q = Seq{__builtin_amdgcn_readlane(l.q.start, at), __builtin_amdgcn_readlane(l.q.n, at),
+                       __builtin_amdgcn_readlane(l.q.len, at)};
             it.ok = true;
             return it;
         }
@@ -321,65 +356,96 @@ __device__ __forceinline__ Col column(const Args &a, const Item &it, int32_t kvh
     return c;
 }
 
-// Q of a column, split; returns the factor that undoes the split's power of two.
+// Q of a column: its loads, and its values split; split() returns the factor
+// that undoes the split's power of two.
 template <int D>
-__device__ __forceinline__ float load_q(const Args &a, const Col &c, int g, h8 (*qh)[2], h8 (*ql)[2])
-{
+struct QRow {
     f4 x[D / 64][4];
-    float mx = 0.f;
+    __device__ __forceinline__ void load(const Args &a, const Col &c, int g)
+    {
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[k][i] = f4{0.f, 0.f, 0.f, 0.f};
-            if (c.token >= 0)
-                x[k][i] = *reinterpret_cast<const f4 *>(a.Q + (int64_t)c.token * a.ldq + c.head * D + 64 * k + 16 * g + 4 * i);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fabsf(x[k][i][u]));
-        }
-    mx = over4_max(mx);
-    const int e = 15 - __builtin_amdgcn_frexp_expf(mx);   // the largest |q| into [2^14, 2^15)
-#pragma unroll
-    for (int k = 0; k < D / 64; ++k)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            uint32_t h[4], l[4];
+        for (int k = 0; k < D / 64; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f4 v = x[k][2 * m + i / 2];
-                split2(ldexpf(v[2 * (i % 2)], e), ldexpf(v[2 * (i % 2) + 1], e), h[i], l[i]);
+                x[k][i] = f4{0.f, 0.f, 0.f, 0.f};
+                if (c.token >= 0)
+                    x[k][i] = *reinterpret_cast<const f4 *>(a.Q + (int64_t)c.token * a.ldq + c.head * D + 64 * k + 16 * g + 4 * i);
             }
-            qh[k][m] = __builtin_bit_cast(h8, u4{h[0], h[1], h[2], h[3]});
-            ql[k][m] = __builtin_bit_cast(h8, u4{l[0], l[1], l[2], l[3]});
-        }
-    return ldexpf(1.0f, -e);
-}
+    }
+    __device__ __forceinline__ float split(h8 (*qh)[2], h8 (*ql)[2]) const
+    {
+        float mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fabsf(x[k][i][u]));
+        const int e = 15 - __builtin_amdgcn_frexp_expf(over4_max(mx));   // the largest |q| into [2^14, 2^15)
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f4 v = x[k][2 * m + i / 2];
+                    split2(ldexpf(v[2 * (i % 2)], e), ldexpf(v[2 * (i % 2) + 1], e), h[i], l[i]);
+                }
+                qh[k][m] = __builtin_bit_cast(h8, u4{h[0], h[1], h[2], h[3]});
+                ql[k][m] = __builtin_bit_cast(h8, u4{l[0], l[1], l[2], l[3]});
+            }
+        return ldexpf(1.0f, -e);
+    }
+};
 
-// 64 groups of 16 tokens of a request from key tile t0 on, lane l the l-th:
-// its place in the cache (in groups; kNone past `end` tokens or outside the
-// cache) and its scales.
+// 64 groups of 16 tokens of a request from key tile t0 on (16 tiles), lane l the
+// l-th: its place in the cache (in groups; kNone past the request's tokens or
+// outside the cache) and its scales.  In two steps, the table's entries and what
+// they lead to, so that a loop over tiles can take them ahead of their use.
 struct Groups {
     uint32_t at;
     float ks, vs;
 };
 
-__device__ __forceinline__ Groups load_groups(const Args &a, int32_t seq, int32_t len, int32_t kvh, int32_t heads,
-                                              int32_t t0)
+__device__ __forceinline__ int32_t load_ids(const Args &a, const Item &it, int32_t t0)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t token = ((int64_t)t0 * 4 + lane) * 16;
+    const int64_t token = ((int64_t)t0 * 4 + (threadIdx.x & 63)) * 16;
+    return token < it.q.len ? a.tables[(int64_t)it.seq * a.width + (token >> a.shift)] : -1;
+}
+
+__device__ __forceinline__ Groups load_groups(const Args &a, int32_t id, int32_t kvh, int32_t heads, int32_t t0)
+{
+    const uint32_t group = (uint32_t)t0 * 4 + (threadIdx.x & 63);   // of 16 tokens, of the request
     Groups r{kNone, 0.f, 0.f};
-    if (token < len) {
-        const int32_t id = a.tables[(int64_t)seq * a.width + (token >> a.shift)];
-        if (id >= 0 && id < a.n_blocks) {
-            const uint32_t block = (uint32_t)id * (uint32_t)heads + (uint32_t)kvh;
-            r.at = (block << (a.shift - 4)) + (uint32_t)((token & ((1 << a.shift) - 1)) >> 4);
-            r.ks = a.ks[block];
-            r.vs = a.vs[block];
-        }
+    if (id >= 0 && id < a.n_blocks) {
+        const uint32_t block = (uint32_t)id * (uint32_t)heads + (uint32_t)kvh;
+        r.at = (block << (a.shift - 4)) + (group & ((1u << (a.shift - 4)) - 1));
+        r.ks = a.ks[block];
+        r.vs = a.vs[block];
     }
     return r;
 }
+
+// The groups of a walk over tiles lo .. hi - 1: advance(t) before tile t's are used.
+struct Walk {
+    Groups now, then;
+    int32_t ids;
+    __device__ __forceinline__ void start(const Args &a, const Item &it, int32_t kvh, int32_t heads, int32_t lo, int32_t id)
+    {
+        now = load_groups(a, id, kvh, heads, lo);
+    }
+    __device__ __forceinline__ void advance(const Args &a, const Item &it, int32_t kvh, int32_t heads, int32_t lo,
+                                            int32_t hi, int32_t t)
+    {
+        const int32_t in = (t - lo) & 15, next = t - in + 16;
+        if (in == 0 && t > lo) now = then;
+        if (next < hi) {
+            if (in == 2) ids = load_ids(a, it, next);
+            if (in == 9) then = load_groups(a, ids, kvh, heads, next);
+        }
+    }
+};
 
 // What a lane needs of its group of a tile.
 struct Lane {
@@ -515,9 +581,39 @@ few_kernel(Args a, int32_t heads)
     const int32_t nt = mine.hi - mine.lo;
     const int32_t t0 = mine.lo + nt * w / 4, t1 = mine.lo + nt * (w + 1) / 4;
 
+    // the table's entries first, then Q: the codes' addresses wait for the former alone
+    const int32_t ids = t0 < t1 ? load_ids(a, it, t0) : -1;
     const Col col = column(a, it, kvh, (int64_t)it.tile * 16 + c);
+    QRow<D> qrow;
+    qrow.load(a, col, g);
+    Walk walk;
+    walk.start(a, it, kvh, heads, t0, ids);
+    // Keys and values of the next tile are loaded as soon as the registers of
+    // this one's are free: half a tile ahead each.
+    u4 kr[4][C], vr[DT];
+    auto load_k = [&](int32_t t) {
+        const uint32_t at = __shfl(walk.now.at, 4 * ((t - t0) & 15) + (c >> 2));
+        const uint8_t *kp = a.k + (size_t)(at == kNone ? 0 : at) * (16 * D) + ((c & 3) * 4 + g) * 16;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < C; ++k) kr[q][k] = *reinterpret_cast<const u4 *>(kp + (q * C + k) * 256);
+    };
+    auto load_v = [&](int32_t t) {
+        const int from = 4 * ((t - t0) & 15) + g;
+        const uint32_t at = __shfl(walk.now.at, from);
+        const uint8_t *vp = a.v + (size_t)(at == kNone ? 0 : at) * (16 * D) + c * 16;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const u4 *>(vp + d * 256);
+        return Lane{__shfl(walk.now.ks, from), __shfl(walk.now.vs, from), at == kNone};
+    };
+    Lane ln{0.f, 0.f, true};
+    if (t0 < t1) {
+        load_k(t0);
+        ln = load_v(t0);
+    }
     h8 qh[C][2], ql[C][2];
-    const float undo = load_q<D>(a, col, g, qh, ql) * a.scale * (MOD ? 1.0f : kLog2e);
+    const float undo = qrow.split(qh, ql) * a.scale * (MOD ? 1.0f : kLog2e);
     // what every (real) query of the wave sees
     int32_t see_lo = col.token >= 0 ? col.lo : 0, see_hi = col.token >= 0 ? col.hi : 0x7FFFFFFF;
 #pragma unroll
@@ -528,24 +624,7 @@ few_kernel(Args a, int32_t heads)
 
     State<D> st;
     st.init();
-    Groups gr{kNone, 0.f, 0.f};
     for (int32_t t = t0; t < t1; ++t) {
-        const int in = (t - t0) & 15;
-        if (in == 0) gr = load_groups(a, it.seq, it.q.len, kvh, heads, t);
-        const uint32_t at_k = __shfl(gr.at, 4 * in + (c >> 2)), at_v = __shfl(gr.at, 4 * in + g);
-        Lane ln;
-        ln.ks = __shfl(gr.ks, 4 * in + g);
-        ln.vs = __shfl(gr.vs, 4 * in + g);
-        ln.none = at_v == kNone;
-        const uint8_t *kp = a.k + (size_t)(at_k == kNone ? 0 : at_k) * (16 * D) + ((c & 3) * 4 + g) * 16;
-        const uint8_t *vp = a.v + (size_t)(at_v == kNone ? 0 : at_v) * (16 * D) + c * 16;
-        u4 kr[4][C], vr[DT];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int k = 0; k < C; ++k) kr[q][k] = *reinterpret_cast<const u4 *>(kp + (q * C + k) * 256);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const u4 *>(vp + d * 256);
         f4 s[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -558,6 +637,10 @@ few_kernel(Args a, int32_t heads)
                     s[q] = mfma(x, qh[k][m], s[q]);
                     s[q] = mfma(x, ql[k][m], s[q]);
                 }
+        }
+        if (t + 1 < t1) {
+            walk.advance(a, it, kvh, heads, t0, t1, t + 1);
+            load_k(t + 1);
         }
         const bool hide = t * 64 < see_lo || (int64_t)t * 64 + 64 > see_hi || __any(ln.none);
         const Weights wt = score_tile<D, MOD>(a, col, ln, t * 64 + 16 * g, undo * ln.ks, hide, s, st);
@@ -574,6 +657,7 @@ few_kernel(Args a, int32_t heads)
             }
         }
         st.l += ldexpf(sum, -(int)wt.e);
+        if (t + 1 < t1) ln = load_v(t + 1);
     }
     // join the waves
     const float l = over4_sum(st.l);
@@ -645,7 +729,9 @@ prompt_kernel(Args a, int32_t heads)
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         col[n] = column(a, it, kvh, (int64_t)it.tile * kPromptRows + 32 * w + 16 * n + c);
-        undo[n] = load_q<D>(a, col[n], g, qh[n], ql[n]) * a.scale * (MOD ? 1.0f : kLog2e);
+        QRow<D> qrow;
+        qrow.load(a, col[n], g);
+        undo[n] = qrow.split(qh[n], ql[n]) * a.scale * (MOD ? 1.0f : kLog2e);
         const bool is = col[n].token >= 0;
         see_lo[n] = is ? col[n].lo : 0;
         see_hi[n] = is ? col[n].hi : 0x7FFFFFFF;
@@ -672,17 +758,18 @@ prompt_kernel(Args a, int32_t heads)
     State<D> st[2];
     st[0].init();
     st[1].init();
-    Groups gr{kNone, 0.f, 0.f};
+    Walk walk;
+    walk.start(a, it, kvh, heads, mine.lo, mine.lo < mine.hi ? load_ids(a, it, mine.lo) : -1);
     u4 kr[C], vr[C];
     // loads tile t (this thread's units of it) and returns what its lane needs of it
     auto load = [&](int32_t t) {
         Lane ln{0.f, 0.f, true};
         if (t >= mine.hi) return ln;
+        walk.advance(a, it, kvh, heads, mine.lo, mine.hi, t);
         const int in = (t - mine.lo) & 15;
-        if (in == 0) gr = load_groups(a, it.seq, it.q.len, kvh, heads, t);
-        const uint32_t at_k = __shfl(gr.at, 4 * in + (c >> 2)), at_v = __shfl(gr.at, 4 * in + g);
-        ln.ks = __shfl(gr.ks, 4 * in + g);
-        ln.vs = __shfl(gr.vs, 4 * in + g);
+        const uint32_t at_k = __shfl(walk.now.at, 4 * in + (c >> 2)), at_v = __shfl(walk.now.at, 4 * in + g);
+        ln.ks = __shfl(walk.now.ks, 4 * in + g);
+        ln.vs = __shfl(walk.now.vs, 4 * in + g);
         ln.none = at_v == kNone;
         const uint8_t *kp = a.k + (size_t)(at_k == kNone ? 0 : at_k) * (16 * D) + ((c & 3) * 4 + g) * 16 + w * 256;
         const uint8_t *vp = a.v + (size_t)(at_v == kNone ? 0 : at_v) * (16 * D) + c * 16 + w * 256;
@@ -778,46 +865,57 @@ prompt_kernel(Args a, int32_t heads)
 }
 
 // ---------------------------------------------------------------- join the parts
-// Workgroup (head fastest): the rows of one row tile that was split, 16 at a
-// time; thread (row, 16 lanes) takes D / 16 of a row's floats.
+// Workgroup (head fastest): 16 rows of one row tile that was split; thread (row,
+// 16 lanes) takes D / 16 of a row's floats.  Four parts' loads are in flight at a time.
 template <int D, int R>
 __global__ void __launch_bounds__(256)
 join_kernel(Args a, int32_t heads)
 {
     const int tid = threadIdx.x;
-    const int32_t kvh = blockIdx.x % heads;
-    const Item it = find_item<R>(a, blockIdx.x / heads, heads, true);
+    const int32_t kvh = blockIdx.x % heads, sub = blockIdx.x / heads % (R / 16);
+    const Item it = find_item<R>(a, blockIdx.x / heads / (R / 16), heads, true);
     if (!it.ok || it.n_split == 1 || (it.part + it.n_split - 1) * heads + kvh >= a.n_part) return;
     const Range all = tile_keys<R>(a, it);
     const int32_t n = all.hi - all.lo, per = (n + it.n_split - 1) / it.n_split;
     const int32_t parts = per ? (n + per - 1) / per : 0;   // the others are empty
-    for (int r0 = 0; r0 < R; r0 += 16) {
-        const int row = r0 + (tid >> 4);
-        const Col out = column(a, it, kvh, (int64_t)it.tile * R + row);
-        if (out.token < 0) continue;
-        float m = -INFINITY;
-        for (int p = 0; p < parts; ++p)
-            m = fmaxf(m, a.part_ml[((int64_t)((it.part + p) * heads + kvh) * R + row) * 2]);
-        f4 x[D / 64];
+    const int row = 16 * sub + (tid >> 4);
+    const Col out = column(a, it, kvh, (int64_t)it.tile * R + row);
+    if (out.token < 0) return;
+    auto index = [&](int32_t p) { return (int64_t)((it.part + min(p, parts - 1)) * heads + kvh) * R + row; };
+    float m = -INFINITY;
+    for (int32_t p = 0; p < parts; p += 16) m = fmaxf(m, a.part_ml[index(p + (tid & 15)) * 2]);
 #pragma unroll
-        for (int d = 0; d < D / 64; ++d) x[d] = f4{0.f, 0.f, 0.f, 0.f};
-        float sum = 0.f;
-        for (int p = 0; p < parts; ++p) {
-            const int64_t at = (int64_t)((it.part + p) * heads + kvh) * R + row;
-            const float d2 = a.part_ml[at * 2] - m;
-            sum += times2(a.part_ml[at * 2 + 1], d2);
+    for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    f4 x[D / 64];
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d) {
-                const f4 y = *reinterpret_cast<const f4 *>(a.part + at * D + 64 * d + 4 * (tid & 15));
+    for (int d = 0; d < D / 64; ++d) x[d] = f4{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    for (int32_t p = 0; p < parts; p += 4) {
+        f4 y[4][D / 64];
+        float ym[4], yl[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) x[d][u] += times2(y[u], d2);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = index(p + i);
+            ym[i] = a.part_ml[at * 2];
+            yl[i] = a.part_ml[at * 2 + 1];
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+                y[i][d] = *reinterpret_cast<const f4 *>(a.part + at * D + 64 * d + 4 * (tid & 15));
         }
-        const float div = sum != 0.f ? 0x1p-15f / sum : 0.f;
-        float *to = a.O + (int64_t)out.token * a.ldo + out.head * D + 4 * (tid & 15);
 #pragma unroll
-        for (int d = 0; d < D / 64; ++d) *reinterpret_cast<f4 *>(to + 64 * d) = x[d] * div;
+        for (int i = 0; i < 4; ++i) {
+            if (p + i >= parts) break;
+            sum += times2(yl[i], ym[i] - m);
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[d][u] += times2(y[i][d][u], ym[i] - m);
+        }
     }
+    const float div = sum != 0.f ? 0x1p-15f / sum : 0.f;
+    float *to = a.O + (int64_t)out.token * a.ldo + out.head * D + 4 * (tid & 15);
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) *reinterpret_cast<f4 *>(to + 64 * d) = x[d] * div;
 }
 
 // ---------------------------------------------------------------- how a call is split
@@ -826,6 +924,8 @@ struct Plan {
     int rows, least;
     int64_t target, tiles, items, parts;   // bounds over one KV head (tiles, items) and over all (parts)
 };
+
+constexpr int64_t kWhole = 16;
 
 Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs,
              int32_t table_width)
@@ -838,11 +938,12 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
     p.target = (few ? 4 : 2) * cus;
     const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
     p.tiles = std::min<int64_t>(n_seqs, rows) + rows * group / p.rows;   // sum of ceil(n_s group / R) over the n_s > 0
-    const int64_t most_split = (most_keys + p.least - 1) / p.least;
-    // sum of tiles * ceil(keys / length) <= tiles + work / length, work / length <= target / heads
-    p.items = std::min(p.tiles * most_split, p.tiles + (p.target + heads - 1) / heads);
+    // up to 16 tiles a row tile's own workgroup does them in less time than a second launch takes
+    const int64_t most_split = most_keys <= kWhole ? 1 : (most_keys + p.least - 1) / p.least;
+    // tiles * ceil(keys / length) <= tiles + work / length and work / length <= target / heads, summed in floats
+    p.items = std::min(p.tiles * most_split, p.tiles + p.target / heads + 2);
     // a tile that is split has more keys than one part, so its parts are at most twice its keys over the length
-    p.parts = most_split <= 1 ? 0 : std::min(p.items * heads, 2 * p.target);
+    p.parts = most_split <= 1 ? 0 : std::min(p.items * heads, 2 * p.target + 4 * heads);
     return p;
 }
 
@@ -854,7 +955,7 @@ template <int FMT, int D, bool MOD>
 int launch(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
 {
     const bool few = p.rows == 16;
-    const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.tiles * heads)), block(256);
+    const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.tiles * heads * (p.rows / 16))), block(256);
     if (few) hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
     else hipLaunchKernelGGL((prompt_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
     if (p.parts) {
@@ -926,7 +1027,7 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     const int64_t need = ml_floats(p) + p.parts * p.rows * kv->head_dim;
     if (need && (!scratch || !aih_kv::aligned16(scratch) || scratch_floats < need)) return AIH_E_INVALID;
     if (rows == 0) return AIH_OK;
-    if (p.items * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
+    if (std::max(p.items, p.tiles * (p.rows / 16)) * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
     Args a{};
     a.k = static_cast<const uint8_t *>(kv->k);
     a.v = static_cast<const uint8_t *>(kv->v);
