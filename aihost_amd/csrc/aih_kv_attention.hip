@@ -44,6 +44,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <type_traits>
 
 namespace {
 
@@ -70,7 +72,7 @@ struct Args {
     int32_t rows, heads, group, n_seqs, width, n_blocks, shift, window;
     int32_t target, least;      // workgroups wanted; the fewest tiles of a part
     int32_t n_part;             // partial tiles that fit the scratch
-    float scale, cap;
+    float scale, cap, inv_group;
 };
 
 // ---------------------------------------------------------------- which part is mine
@@ -89,7 +91,7 @@ __device__ __forceinline__ Seq seq_of(const Args &a, int s)
 template <int R>
 __device__ __forceinline__ int32_t row_tiles(const Args &a, const Seq &q)
 {
-    return (int32_t)(((int64_t)q.n * a.group + R - 1) / R);
+    return (int32_t)(((uint32_t)q.n * (uint32_t)a.group + R - 1) / R);
 }
 __device__ __forceinline__ int32_t key_tiles(const Args &a, const Seq &q)
 {
@@ -210,21 +212,32 @@ __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t he
     return none;
 }
 
+// What a request's queries see: position p the keys max(0, p - window + 1) ..
+// min(max(p + 1, prefix), len) - 1.
+struct View {
+    int32_t prefix, len, window;
+    __device__ __forceinline__ int32_t lo(int32_t p) const { return window > 0 ? max(0, p - window + 1) : 0; }
+    __device__ __forceinline__ int32_t hi(int32_t p) const { return min(max(p + 1, prefix), len); }
+};
+
+__device__ __forceinline__ View view_of(const Args &a, const Item &it)
+{
+    return View{a.prefix ? a.prefix[it.seq] : 0, it.q.len, a.window};
+}
+
 // The key tiles of a row tile, and of its part `split`: an equal share each.
 struct Range {
     int32_t lo, hi;
 };
 
 template <int R>
-__device__ __forceinline__ Range tile_keys(const Args &a, const Item &it)
+__device__ __forceinline__ Range tile_keys(const Args &a, const Item &it, const View &v)
 {
-    const int64_t f0 = (int64_t)it.tile * R, f1 = min<int64_t>(f0 + R, (int64_t)it.q.n * a.group) - 1;
+    const uint32_t f0 = (uint32_t)it.tile * R;
     const int32_t base = it.q.len - it.q.n;
-    const int32_t p0 = base + (int32_t)(f0 / a.group), p1 = base + (int32_t)(f1 / a.group);
-    int32_t end = p1 + 1;
-    if (a.prefix) end = max(end, a.prefix[it.seq]);
-    end = min(end, it.q.len);
-    const int32_t lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+    const int32_t p0 = base + (int32_t)(f0 / (uint32_t)a.group);
+    const int32_t p1 = base + min((int32_t)((f0 + R - 1) / (uint32_t)a.group), it.q.n - 1);
+    const int32_t end = v.hi(p1), lo = v.lo(p0);
     return Range{lo / 64, end <= lo ? lo / 64 : (int32_t)(((int64_t)end + 63) / 64)};
 }
 
@@ -266,7 +279,8 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
 {
     const f2 x = {x0, x1};
     const h2 h = __builtin_convertvector(x, h2);
-    const h2 l = __builtin_convertvector(x - __builtin_convertvector(h, f2), h2);
+    const f2 r = {fmaf(-(float)h[0], 1.0f, x0), fmaf(-(float)h[1], 1.0f, x1)};   // one v_fma_mix each
+    const h2 l = __builtin_convertvector(r, h2);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, l);
 }
@@ -332,28 +346,69 @@ struct State {
     }
 };
 
-// The query of a column: its place among the rows and what it sees.
+// The query of a column: its position (kNobody for a column past the request's
+// rows, which is computed and not stored) and the slope of its head, times log2 e.
+constexpr int32_t kNobody = -0x40000000;
 struct Col {
-    int32_t token, head;   // query row (of Q and O), head; token -1: none
-    int32_t pos, lo, hi;   // position; keys lo .. hi - 1 are seen
-    float slope;           // of its head, times log2 e
+    int32_t pos;
+    float slope;
 };
 
-__device__ __forceinline__ Col column(const Args &a, const Item &it, int32_t kvh, int64_t f)
+// Row f0 + x of a request (f0 the first of a tile, x < 128): its token and its
+// head within the group.  The quotient of the remainder is taken in floats, exact
+// below 2^21: it lies half a step or more from an integer.
+struct Place {
+    int32_t token, head;
+};
+
+__device__ __forceinline__ Place place_of(const Args &a, uint32_t f0, uint32_t x)
 {
-    Col c{-1, 0, 0, 0, 0, 0.f};
-    if (f < (int64_t)it.q.n * a.group) {
-        const int32_t i = (int32_t)(f / a.group);
-        c.token = it.q.start + i;
-        c.head = kvh * a.group + (int32_t)(f % a.group);
-        c.pos = it.q.len - it.q.n + i;
-        c.hi = c.pos + 1;
-        if (a.prefix) c.hi = max(c.hi, a.prefix[it.seq]);
-        c.hi = min(c.hi, it.q.len);
-        c.lo = a.window > 0 ? max(0, c.pos - a.window + 1) : 0;
-        if (a.slopes) c.slope = a.slopes[c.head] * kLog2e;
+    const uint32_t t0 = f0 / (uint32_t)a.group, r = f0 - t0 * (uint32_t)a.group + x;
+    const uint32_t t = (uint32_t)(((float)r + 0.5f) * a.inv_group);
+    return Place{(int32_t)(t0 + t), (int32_t)(r - t * (uint32_t)a.group)};
+}
+
+// Where the row's values lie: its query row, -1 for none, and its head.
+__device__ __forceinline__ Place row_of(const Args &a, const Item &it, int32_t kvh, uint32_t f0, uint32_t x)
+{
+    const Place p = place_of(a, f0, x);
+    return Place{p.token < it.q.n ? it.q.start + p.token : -1, kvh * a.group + p.head};
+}
+
+__device__ __forceinline__ Col column(const Args &a, const Item &it, const Place &row)
+{
+    Col c{kNobody, 0.f};
+    if (row.token >= 0) {
+        c.pos = it.q.len - it.q.n + (row.token - it.q.start);
+        if (a.slopes) c.slope = a.slopes[row.head] * kLog2e;
     }
     return c;
+}
+
+// Key tiles by what the queries of 16 columns see of them: all of them see
+// all keys of tiles all_lo .. all_hi - 1, some of them some keys of tiles any_lo .. any_hi - 1.
+struct Sight {
+    int32_t all_lo, all_hi, any_lo, any_hi;
+};
+
+__device__ __forceinline__ Sight sight_of(const View &v, const Col &c)
+{
+    const bool is = c.pos != kNobody;
+    int32_t lo0 = is ? v.lo(c.pos) : 0, lo1 = is ? lo0 : 0x7FFFFFFF;   // largest and smallest
+    int32_t hi0 = is ? v.hi(c.pos) : 0x7FFFFFFF, hi1 = is ? hi0 : 0;   // smallest and largest
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        lo0 = max(lo0, __shfl_xor(lo0, d));
+        lo1 = min(lo1, __shfl_xor(lo1, d));
+        hi0 = min(hi0, __shfl_xor(hi0, d));
+        hi1 = max(hi1, __shfl_xor(hi1, d));
+    }
+    lo0 = __builtin_amdgcn_readfirstlane(lo0);
+    lo1 = __builtin_amdgcn_readfirstlane(lo1);
+    hi0 = __builtin_amdgcn_readfirstlane(hi0);
+    hi1 = __builtin_amdgcn_readfirstlane(hi1);
+    // hi may be 0 or less for a query that sees nothing
+    return Sight{(int32_t)(((uint32_t)lo0 + 63) / 64), hi0 > 0 ? hi0 / 64 : 0, lo1 / 64, hi1 > 0 ? (int32_t)(((uint32_t)hi1 + 63) / 64) : 0};
 }
 
 // Q of a column: its loads, and its values split; split() returns the factor
@@ -361,7 +416,7 @@ __device__ __forceinline__ Col column(const Args &a, const Item &it, int32_t kvh
 template <int D>
 struct QRow {
     f4 x[D / 64][4];
-    __device__ __forceinline__ void load(const Args &a, const Col &c, int g)
+    __device__ __forceinline__ void load(const Args &a, const Place &c, int g)
     {
 #pragma unroll
         for (int k = 0; k < D / 64; ++k)
@@ -403,6 +458,7 @@ struct QRow {
 // l-th: its place in the cache (in groups; kNone past the request's tokens or
 // outside the cache) and its scales.  In two steps, the table's entries and what
 // they lead to, so that a loop over tiles can take them ahead of their use.
+constexpr float kHidden = -1.0f;   // the value scale of a group that is not there
 struct Groups {
     uint32_t at;
     float ks, vs;
@@ -417,7 +473,7 @@ __device__ __forceinline__ int32_t load_ids(const Args &a, const Item &it, int32
 __device__ __forceinline__ Groups load_groups(const Args &a, int32_t id, int32_t kvh, int32_t heads, int32_t t0)
 {
     const uint32_t group = (uint32_t)t0 * 4 + (threadIdx.x & 63);   // of 16 tokens, of the request
-    Groups r{kNone, 0.f, 0.f};
+    Groups r{kNone, 0.f, kHidden};
     if (id >= 0 && id < a.n_blocks) {
         const uint32_t block = (uint32_t)id * (uint32_t)heads + (uint32_t)kvh;
         r.at = (block << (a.shift - 4)) + (group & ((1u << (a.shift - 4)) - 1));
@@ -447,10 +503,9 @@ struct Walk {
     }
 };
 
-// What a lane needs of its group of a tile.
+// What a lane needs of its group of a tile: the scales.
 struct Lane {
-    float ks, vs;   // scales
-    bool none;      // the group is not there
+    float ks, vs;
 };
 
 // What makes weights of a lane's products of one tile: p = 2^(f s + add), the
@@ -464,8 +519,8 @@ struct Weights {
 // tile + 16 g); f: the factor that makes them scores, times log2 e unless MOD.
 // hide (the same in all lanes): some key of the tile is not seen by some query.
 template <int D, bool MOD>
-__device__ __forceinline__ Weights score_tile(const Args &a, const Col &c, const Lane &ln, int32_t key0, float f,
-                                              bool hide, f4 *s, State<D> &st)
+__device__ __forceinline__ Weights score_tile(const Args &a, const View &v, const Col &c, const Lane &ln, int32_t key0,
+                                              float f, bool hide, f4 *s, State<D> &st)
 {
     if constexpr (MOD) {
         float top = 0.f;
@@ -498,10 +553,10 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const Col &c, const
             for (int i = 0; i < 4; ++i) s[t][i] = fmaf(-c.slope, fabsf(far - (float)(4 * t + i)), s[t][i]);
         f = 1.0f;
     }
-    bool some = true;   // the query sees a key of this lane's group
+    float scale = ln.vs;   // 0 where the query sees no key of this lane's group: that block may have no number for a scale
     if (hide) {
-        const int32_t lo = c.lo - key0, hi = ln.none ? -1 : c.hi - key0;
-        some = lo < 16 && hi > 0;
+        const int32_t lo = v.lo(c.pos) - key0, hi = ln.vs == kHidden ? -1 : v.hi(c.pos) - key0;
+        if (!(lo < 16 && hi > 0)) scale = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -511,10 +566,10 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const Col &c, const
             }
         f = 1.0f;
     }
-    const float ve = ln.vs > 0.f && ln.vs < INFINITY ? (float)__builtin_amdgcn_frexp_expf(ln.vs) : kNoExp;
-    st.e = fmaxf(st.e, over4_max(some ? ve : kNoExp));
+    const float ve = scale > 0.f && scale < INFINITY ? (float)__builtin_amdgcn_frexp_expf(scale) : kNoExp;
+    st.e = fmaxf(st.e, over4_max(ve));
     const float e = st.e == kNoExp ? 0.f : fmaxf(fmaxf(ve, st.e - 60.f), -100.f);
-    const float vs = ldexpf(ln.vs, 15 - (int)e);
+    const float vs = ldexpf(scale, 15 - (int)e);
     float mx = s[0][0];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -541,7 +596,7 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const Col &c, const
 }
 
 // The weights of keys 8 m + 0..7 of the lane's group, split; the sum of their p is added to `sum`.
-__device__ __forceinline__ void weigh(const Weights &w, bool hide, int m, const f4 *s, float &sum, h8 &ph, h8 &pl)
+__device__ __forceinline__ void weigh(const Weights &w, int m, const f4 *s, float &sum, h8 &ph, h8 &pl)
 {
     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -550,12 +605,7 @@ __device__ __forceinline__ void weigh(const Weights &w, bool hide, int m, const 
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s0, w.f, w.add)), p1 = __builtin_amdgcn_exp2f(fmaf(s1, w.f, w.add));
         sum += p0;
         sum += p1;
-        float w0 = p0 * w.vs, w1 = p1 * w.vs;
-        if (hide) {   // a hidden key's block may have no number for a scale
-            w0 = s0 == -INFINITY ? 0.f : w0;
-            w1 = s1 == -INFINITY ? 0.f : w1;
-        }
-        split2(w0, w1, hi[i], lo[i]);
+        split2(p0 * w.vs, p1 * w.vs, hi[i], lo[i]);
     }
     ph = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
     pl = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
@@ -577,15 +627,17 @@ few_kernel(Args a, int32_t heads)
     const int32_t kvh = blockIdx.x % heads;
     const Item it = find_item<16>(a, blockIdx.x / heads, heads, false);
     if (!it.ok) return;
-    const Range all = tile_keys<16>(a, it), mine = part_of(all, it.split, it.n_split);
+    const View view = view_of(a, it);
+    const Range all = tile_keys<16>(a, it, view), mine = part_of(all, it.split, it.n_split);
     const int32_t nt = mine.hi - mine.lo;
     const int32_t t0 = mine.lo + nt * w / 4, t1 = mine.lo + nt * (w + 1) / 4;
 
     // the table's entries first, then Q: the codes' addresses wait for the former alone
     const int32_t ids = t0 < t1 ? load_ids(a, it, t0) : -1;
-    const Col col = column(a, it, kvh, (int64_t)it.tile * 16 + c);
+    const Place place = row_of(a, it, kvh, (uint32_t)it.tile * 16, c);
     QRow<D> qrow;
-    qrow.load(a, col, g);
+    qrow.load(a, place, g);
+    const Col col = column(a, it, place);
     Walk walk;
     walk.start(a, it, kvh, heads, t0, ids);
     // Keys and values of the next tile are loaded as soon as the registers of
@@ -605,22 +657,16 @@ few_kernel(Args a, int32_t heads)
         const uint8_t *vp = a.v + (size_t)(at == kNone ? 0 : at) * (16 * D) + c * 16;
 #pragma unroll
         for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const u4 *>(vp + d * 256);
-        return Lane{__shfl(walk.now.ks, from), __shfl(walk.now.vs, from), at == kNone};
+        return Lane{__shfl(walk.now.ks, from), __shfl(walk.now.vs, from)};
     };
-    Lane ln{0.f, 0.f, true};
+    Lane ln{0.f, kHidden};
     if (t0 < t1) {
         load_k(t0);
         ln = load_v(t0);
     }
     h8 qh[C][2], ql[C][2];
     const float undo = qrow.split(qh, ql) * a.scale * (MOD ? 1.0f : kLog2e);
-    // what every (real) query of the wave sees
-    int32_t see_lo = col.token >= 0 ? col.lo : 0, see_hi = col.token >= 0 ? col.hi : 0x7FFFFFFF;
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-        see_lo = max(see_lo, __shfl_xor(see_lo, d));
-        see_hi = min(see_hi, __shfl_xor(see_hi, d));
-    }
+    const Sight sight = sight_of(view, col);
 
     State<D> st;
     st.init();
@@ -642,13 +688,13 @@ few_kernel(Args a, int32_t heads)
             walk.advance(a, it, kvh, heads, t0, t1, t + 1);
             load_k(t + 1);
         }
-        const bool hide = t * 64 < see_lo || (int64_t)t * 64 + 64 > see_hi || __any(ln.none);
-        const Weights wt = score_tile<D, MOD>(a, col, ln, t * 64 + 16 * g, undo * ln.ks, hide, s, st);
+        const bool hide = t < sight.all_lo || t >= sight.all_hi || __any(ln.vs == kHidden);
+        const Weights wt = score_tile<D, MOD>(a, view, col, ln, t * 64 + 16 * g, undo * ln.ks, hide, s, st);
         float sum = 0.f;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             h8 ph, pl;
-            weigh(wt, hide, m, s, sum, ph, pl);
+            weigh(wt, m, s, sum, ph, pl);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const h8 x = to_half<FMT>(vr[d][2 * m], vr[d][2 * m + 1]);
@@ -676,7 +722,7 @@ few_kernel(Args a, int32_t heads)
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += times2(ls[i][row], ms[i][row] - m);
     const bool whole = it.n_split == 1;
-    const Col out = column(a, it, kvh, (int64_t)it.tile * 16 + row);
+    const Place out = row_of(a, it, kvh, (uint32_t)it.tile * 16, row);
     const int32_t part = (it.part + it.split) * heads + kvh;
     if (!whole && part >= a.n_part) return;   // never: the scratch is sized for every part
     const float div = !whole ? 1.0f : sum != 0.f ? 0x1p-15f / sum : 0.f;
@@ -699,78 +745,47 @@ few_kernel(Args a, int32_t heads)
     }
 }
 
-// ---------------------------------------------------------------- many rows: 128 at a time
-constexpr int kPromptRows = 128;
-
-// Workgroup (head fastest): a part of one tile of 128 rows, 32 to a wave.  The
-// codes of a key tile are converted to fp16 once, into LDS, in the order in
-// which the lanes read them (unit by unit, so every LDS access is 1 KB in a row),
-// and every fragment read feeds the four products of two column tiles and
-// two halves.  Two images: while a tile is multiplied, the next one, loaded a tile
+// ---------------------------------------------------------------- many rows: 64 or 128 at a time
+// Workgroup (head fastest): a part of one tile of 64 N rows, N columns of 16 to
+// a wave.  The codes of a key tile are converted to fp16 once, into LDS, in the
+// order in which the lanes read them (unit by unit, so every LDS access is 1 KB in
+// a row), and every fragment read feeds the products of N columns and two
+// halves.  Two images: while a tile is multiplied, the next one, loaded a tile
 // ago, is converted, and the one after it is loaded.  One barrier per tile.
-template <int FMT, int D, bool MOD>
+template <int FMT, int D, int N, bool MOD>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 prompt_kernel(Args a, int32_t heads)
 {
-    constexpr int C = D / 64, DT = D / 16;
+    constexpr int C = D / 64, DT = D / 16, FR = 8 * C, R = 64 * N;
     __shared__ h8 image[2][2][4 * C * 2 * 64];   // [buffer][keys, values][(unit row, half)][lane]
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int32_t kvh = blockIdx.x % heads;
-    const Item it = find_item<kPromptRows>(a, blockIdx.x / heads, heads, false);
+    const Item it = find_item<R>(a, blockIdx.x / heads, heads, false);
     if (!it.ok) return;
-    const Range all = tile_keys<kPromptRows>(a, it), mine = part_of(all, it.split, it.n_split);
+    const View view = view_of(a, it);
+    const Range all = tile_keys<R>(a, it, view), mine = part_of(all, it.split, it.n_split);
 
-    Col col[2];
-    h8 qh[2][C][2], ql[2][C][2];
-    float undo[2];
-    int32_t see_lo[2], see_hi[2];               // what every query of a column tile sees
-    int32_t any_lo = 0x7FFFFFFF, any_hi = 0;    // and any of the wave's
+    // the table's entries first, then Q: the codes' addresses wait for the former alone
+    const int32_t ids = mine.lo < mine.hi ? load_ids(a, it, mine.lo) : -1;
+    Col col[N];
+    QRow<D> qrow[N];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        col[n] = column(a, it, kvh, (int64_t)it.tile * kPromptRows + 32 * w + 16 * n + c);
-        QRow<D> qrow;
-        qrow.load(a, col[n], g);
-        undo[n] = qrow.split(qh[n], ql[n]) * a.scale * (MOD ? 1.0f : kLog2e);
-        const bool is = col[n].token >= 0;
-        see_lo[n] = is ? col[n].lo : 0;
-        see_hi[n] = is ? col[n].hi : 0x7FFFFFFF;
-        if (is) {
-            any_lo = min(any_lo, col[n].lo);
-            any_hi = max(any_hi, col[n].hi);
-        }
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            see_lo[n] = max(see_lo[n], __shfl_xor(see_lo[n], d));
-            see_hi[n] = min(see_hi[n], __shfl_xor(see_hi[n], d));
-        }
-        see_lo[n] = __builtin_amdgcn_readfirstlane(see_lo[n]);
-        see_hi[n] = __builtin_amdgcn_readfirstlane(see_hi[n]);
+    for (int n = 0; n < N; ++n) {
+        const Place place = row_of(a, it, kvh, (uint32_t)it.tile * R, 16 * N * w + 16 * n + c);
+        qrow[n].load(a, place, g);
+        col[n] = column(a, it, place);
     }
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-        any_lo = min(any_lo, __shfl_xor(any_lo, d));
-        any_hi = max(any_hi, __shfl_xor(any_hi, d));
-    }
-    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
-    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-
-    State<D> st[2];
-    st[0].init();
-    st[1].init();
     Walk walk;
-    walk.start(a, it, kvh, heads, mine.lo, mine.lo < mine.hi ? load_ids(a, it, mine.lo) : -1);
-    u4 kr[C], vr[C];
+    walk.start(a, it, kvh, heads, mine.lo, ids);
+    u4 kr[C] = {}, vr[C] = {};
     // loads tile t (this thread's units of it) and returns what its lane needs of it
     auto load = [&](int32_t t) {
-        Lane ln{0.f, 0.f, true};
+        Lane ln{0.f, kHidden};
         if (t >= mine.hi) return ln;
         walk.advance(a, it, kvh, heads, mine.lo, mine.hi, t);
         const int in = (t - mine.lo) & 15;
         const uint32_t at_k = __shfl(walk.now.at, 4 * in + (c >> 2)), at_v = __shfl(walk.now.at, 4 * in + g);
-        ln.ks = __shfl(walk.now.ks, 4 * in + g);
-        ln.vs = __shfl(walk.now.vs, 4 * in + g);
-        ln.none = at_v == kNone;
         const uint8_t *kp = a.k + (size_t)(at_k == kNone ? 0 : at_k) * (16 * D) + ((c & 3) * 4 + g) * 16 + w * 256;
         const uint8_t *vp = a.v + (size_t)(at_v == kNone ? 0 : at_v) * (16 * D) + c * 16 + w * 256;
 #pragma unroll
@@ -778,6 +793,8 @@ prompt_kernel(Args a, int32_t heads)
             kr[i] = *reinterpret_cast<const u4 *>(kp + i * 1024);
             vr[i] = *reinterpret_cast<const u4 *>(vp + i * 1024);
         }
+        ln.ks = __shfl(walk.now.ks, 4 * in + g);
+        ln.vs = __shfl(walk.now.vs, 4 * in + g);
         return ln;
     };
     auto convert = [&](int b) {
@@ -790,70 +807,103 @@ prompt_kernel(Args a, int32_t heads)
             }
     };
     Lane ln = load(mine.lo), next{};
-    if (mine.lo < mine.hi) convert(0);
+    Sight sight[N];
+    h8 qh[N][C][2], ql[N][C][2];
+    float undo[N];
+    State<D> st[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        undo[n] = qrow[n].split(qh[n], ql[n]) * a.scale * (MOD ? 1.0f : kLog2e);
+        sight[n] = sight_of(view, col[n]);
+        st[n].init();
+    }
+    convert(0);
     next = load(mine.lo + 1);
     __syncthreads();
-    for (int32_t t = mine.lo; t < mine.hi; ++t) {
-        const int b = (t - mine.lo) & 1;
-        const bool work = t * 64 < any_hi && (int64_t)t * 64 + 64 > any_lo;
-        f4 s[2][4];
-        Weights wt[2];
-        bool hide[2] = {false, false};
-        if (work) {
+    // tile t, in buffer B (a constant: reads of one buffer and writes of the other may then pass each other)
+    auto step = [&](auto buffer, int32_t t) {
+        constexpr int b = decltype(buffer)::value;
+        f4 s[N][4];
+        {
+            const h8 *x = &image[b][0][lane];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                s[0][q] = s[1][q] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < FR; ++i) {   // fragment i: key rows q = i / (2 C), dimensions (k, m)
+                const int q = i / (2 * C), k = i / 2 % C, m = i % 2;
+                const h8 f = x[i * 64];
 #pragma unroll
-                for (int k = 0; k < C; ++k)
+                for (int n = 0; n < N; ++n) s[n][q] = mfma(f, qh[n][k][m], i % (2 * C) ? s[n][q] : f4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const h8 x = image[b][0][((q * C + k) * 2 + m) * 64 + lane];
-                        s[0][q] = mfma(x, qh[0][k][m], s[0][q]);
-                        s[1][q] = mfma(x, qh[1][k][m], s[1][q]);
-                        s[0][q] = mfma(x, ql[0][k][m], s[0][q]);
-                        s[1][q] = mfma(x, ql[1][k][m], s[1][q]);
-                    }
+                for (int n = 0; n < N; ++n) s[n][q] = mfma(f, ql[n][k][m], s[n][q]);
             }
-            const bool none = __any(ln.none);
+            // Left alone, the compiler reads a fragment, waits for it and multiplies: 306 us where reading three ahead
+            // takes 283 (four prompts of 363 to 3690 tokens, 32 heads over 8, e4m3).
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                hide[n] = none || t * 64 < see_lo[n] || (int64_t)t * 64 + 64 > see_hi[n];
-                wt[n] = score_tile<D, MOD>(a, col[n], ln, t * 64 + 16 * g, undo[n] * ln.ks, hide[n], s[n], st[n]);
+            for (int i = 0; i < FR; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * N, 0);
+                if (i + 3 < FR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         }
-        if (t + 1 < mine.hi) convert(b ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        convert(b ^ 1);   // of tile t + 1; past the last tile, of what was there, for nobody
+        const Lane here = ln;
         ln = next;
         next = load(t + 2);
-        if (work) {
-            float sum[2] = {0.f, 0.f};
+        const bool none = __any(here.vs == kHidden);
+        Weights wt[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const bool hide = none || t < sight[n].all_lo || t >= sight[n].all_hi;
+            wt[n] = score_tile<D, MOD>(a, view, col[n], here, t * 64 + 16 * g, undo[n] * here.ks, hide, s[n], st[n]);
+        }
+        {
+            const h8 *x = &image[b][1][lane];
+            float sum[N] = {};
+            h8 ph[N], pl[N];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                h8 ph[2], pl[2];
-                weigh(wt[0], hide[0], m, s[0], sum[0], ph[0], pl[0]);
-                weigh(wt[1], hide[1], m, s[1], sum[1], ph[1], pl[1]);
+#pragma unroll
+                for (int n = 0; n < N; ++n) weigh(wt[n], m, s[n], sum[n], ph[n], pl[n]);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const h8 x = image[b][1][(d * 2 + m) * 64 + lane];
-                    st[0].o[d] = mfma(x, ph[0], st[0].o[d]);
-                    st[1].o[d] = mfma(x, ph[1], st[1].o[d]);
-                    st[0].o[d] = mfma(x, pl[0], st[0].o[d]);
-                    st[1].o[d] = mfma(x, pl[1], st[1].o[d]);
+                    const h8 f = x[(d * 2 + m) * 64];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) st[n].o[d] = mfma(f, ph[n], st[n].o[d]);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) st[n].o[d] = mfma(f, pl[n], st[n].o[d]);
                 }
             }
-            st[0].l += ldexpf(sum[0], -(int)wt[0].e);
-            st[1].l += ldexpf(sum[1], -(int)wt[1].e);
+#pragma unroll
+            for (int n = 0; n < N; ++n) st[n].l += ldexpf(sum[n], -(int)wt[n].e);
+            // the first half's weights, then its products with the second half's weights between them
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 1);
+            __builtin_amdgcn_sched_group_barrier(0x402, 58 * N, 1);
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, N, 1);
+                if (i < DT) __builtin_amdgcn_sched_group_barrier(0x402, 56 * N / (2 * DT), 1);
+                __builtin_amdgcn_sched_group_barrier(0x008, N, 1);
+                if (i + 3 < 2 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+                if (i < DT) __builtin_amdgcn_sched_group_barrier(0x402, 56 * N / (2 * DT), 1);
+            }
         }
         __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int32_t t = mine.lo; t < mine.hi; t += 2) {
+        step(std::integral_constant<int, 0>(), t);
+        if (t + 1 < mine.hi) step(std::integral_constant<int, 1>(), t + 1);
     }
     const bool whole = it.n_split == 1;
     const int32_t part = (it.part + it.split) * heads + kvh;
     if (!whole && part >= a.n_part) return;   // never: the scratch is sized for every part
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < N; ++n) {
         const float sum = over4_sum(st[n].l);
-        if (col[n].token < 0) continue;
-        const int64_t row = (int64_t)part * kPromptRows + 32 * w + 16 * n + c;
-        float *to = whole ? a.O + (int64_t)col[n].token * a.ldo + col[n].head * D : a.part + row * D;
+        const Place out = row_of(a, it, kvh, (uint32_t)it.tile * R, 16 * N * w + 16 * n + c);
+        if (out.token < 0) continue;
+        const int64_t row = (int64_t)part * R + 16 * N * w + 16 * n + c;
+        float *to = whole ? a.O + (int64_t)out.token * a.ldo + out.head * D : a.part + row * D;
         if (!whole && g == 0) {
             a.part_ml[row * 2] = st[n].m;
             a.part_ml[row * 2 + 1] = sum;
@@ -875,11 +925,11 @@ join_kernel(Args a, int32_t heads)
     const int32_t kvh = blockIdx.x % heads, sub = blockIdx.x / heads % (R / 16);
     const Item it = find_item<R>(a, blockIdx.x / heads / (R / 16), heads, true);
     if (!it.ok || it.n_split == 1 || (it.part + it.n_split - 1) * heads + kvh >= a.n_part) return;
-    const Range all = tile_keys<R>(a, it);
+    const Range all = tile_keys<R>(a, it, view_of(a, it));
     const int32_t n = all.hi - all.lo, per = (n + it.n_split - 1) / it.n_split;
     const int32_t parts = per ? (n + per - 1) / per : 0;   // the others are empty
     const int row = 16 * sub + (tid >> 4);
-    const Col out = column(a, it, kvh, (int64_t)it.tile * R + row);
+    const Place out = row_of(a, it, kvh, (uint32_t)it.tile * R, row);
     if (out.token < 0) return;
     auto index = [&](int32_t p) { return (int64_t)((it.part + min(p, parts - 1)) * heads + kvh) * R + row; };
     float m = -INFINITY;
@@ -933,9 +983,13 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
     const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256, heads = kv->n_kv_heads, group = n_heads / heads;
     Plan p{};
     const bool few = rows * group <= 32 * (int64_t)n_seqs;
-    p.rows = few ? 16 : kPromptRows;
+    const bool wide = kv->head_dim < 256 && rows * group * heads >= 128 * cus;
+    p.rows = few ? 16 : wide ? 128 : 64;
     p.least = 4;
-    p.target = (few ? 4 : 2) * cus;
+    p.target = few ? (kv->head_dim == 256 ? 1 : kv->head_dim == 128 ? 4 : 2) * cus : (kv->head_dim == 256 ? 1 : 2) * cus;
+    if (getenv("T_ROWS")) p.rows = atoi(getenv("T_ROWS"));
+    if (getenv("T_TARGET")) p.target = atoi(getenv("T_TARGET"));
+    if (getenv("T_LEAST")) p.least = atoi(getenv("T_LEAST"));
     const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
     p.tiles = std::min<int64_t>(n_seqs, rows) + rows * group / p.rows;   // sum of ceil(n_s group / R) over the n_s > 0
     // up to 16 tiles a row tile's own workgroup does them in less time than a second launch takes
@@ -954,15 +1008,17 @@ int64_t ml_floats(const Plan &p) { return (p.parts * p.rows * 2 + kAlign - 1) / 
 template <int FMT, int D, bool MOD>
 int launch(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
 {
-    const bool few = p.rows == 16;
     const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.tiles * heads * (p.rows / 16))), block(256);
-    if (few) hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
-    else hipLaunchKernelGGL((prompt_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
+    constexpr int kWide = D == 256 ? 1 : 2;   // at D = 256 a wave's registers hold one column of 16
+    if (p.rows == 16) hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
+    else if (p.rows == 64) hipLaunchKernelGGL((prompt_kernel<FMT, D, 1, MOD>), grid, block, 0, ctx->stream, a, heads);
+    else hipLaunchKernelGGL((prompt_kernel<FMT, D, kWide, MOD>), grid, block, 0, ctx->stream, a, heads);
     if (p.parts) {
         const int rc = aih_launch_status();
         if (rc) return rc;
-        if (few) hipLaunchKernelGGL((join_kernel<D, 16>), join, block, 0, ctx->stream, a, heads);
-        else hipLaunchKernelGGL((join_kernel<D, kPromptRows>), join, block, 0, ctx->stream, a, heads);
+        if (p.rows == 16) hipLaunchKernelGGL((join_kernel<D, 16>), join, block, 0, ctx->stream, a, heads);
+        else if (p.rows == 64) hipLaunchKernelGGL((join_kernel<D, 64>), join, block, 0, ctx->stream, a, heads);
+        else hipLaunchKernelGGL((join_kernel<D, 64 * kWide>), join, block, 0, ctx->stream, a, heads);
     }
     return aih_launch_status();
 }
@@ -987,7 +1043,7 @@ int check_batch(const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n
 {
     if (n_heads <= 0 || rows < 0 || n_seqs <= 0 || table_width <= 0 || n_heads % kv->n_kv_heads) return AIH_E_INVALID;
     if (n_seqs > aih_kv::kMaxSeqs || (int64_t)table_width * kv->block_tokens > 0x7FFFFFFF || rows > 0x7FFFFFFF ||
-        rows * n_heads > (int64_t)1 << 33 || n_heads > 1 << 20)
+        rows * (n_heads / kv->n_kv_heads) > 0x7FFFFF00 || n_heads > 1 << 20)
         return AIH_E_LIMIT;
     return AIH_OK;
 }
@@ -1047,6 +1103,7 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     a.rows = (int32_t)rows;
     a.heads = n_heads;
     a.group = n_heads / kv->n_kv_heads;
+    a.inv_group = 1.0f / (float)a.group;
     a.n_seqs = n_seqs;
     a.width = table_width;
     a.n_blocks = kv->n_blocks;
