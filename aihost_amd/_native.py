@@ -137,6 +137,7 @@ SIGNATURES = {
     "aih_kv_append_rope": (_i, [_vp, _kvp, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i32]),
     "aih_kv_read": (_i, [_vp, _kvp, _vp, _i64, _vp, _i64, _vp, _i64]),
     "aih_kv_attention_scratch_floats": (_i64, [_vp, _kvp, _i32, _i64, _i32, _i32]),
+    "aih_kv_attention_tile_rows": (_i, [_vp, _kvp, _i32, _i64, _i32, _i32]),
     "aih_kv_attention": (_i, [_vp, _kvp, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _f, _scp, _vp,
                               _i64]),
     "aih_sync": (_i, [_vp]),

@@ -44,7 +44,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 namespace {
@@ -167,9 +166,13 @@ __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t he
             work += (float)l.tiles * (float)l.keys;
             tiles_all += (float)l.tiles;
         }
-        const float want = (float)a.target / (float)heads;
+        float want = (float)a.target / (float)heads;
+        tiles_all = wave_add(tiles_all);
+        // about as many tiles as workgroups wanted, and of different lengths: shorter parts even them out (64 requests of
+        // 512 to 7804 tokens, 512 wanted: 94.7 -> 87.3 us)
+        if (tiles_all > 0.75f * want) want *= 2.0f;
         len = max(a.least, (int32_t)ceilf(wave_add(work) / want));
-        if (wave_add(tiles_all) < want) {
+        if (tiles_all < want) {
             for (int i = 0; i < 4; ++i) {
                 float n = (float)first.tiles * (float)((first.keys + len - 1) / len);
                 for (int base = 64; base < a.n_seqs; base += 64) {
@@ -797,14 +800,11 @@ prompt_kernel(Args a, int32_t heads)
         ln.vs = __shfl(walk.now.vs, 4 * in + g);
         return ln;
     };
-    auto convert = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                image[b][0][((w + 4 * i) * 2 + m) * 64 + lane] = to_half<FMT>(kr[i][2 * m], kr[i][2 * m + 1]);
-                image[b][1][((w + 4 * i) * 2 + m) * 64 + lane] = to_half<FMT>(vr[i][2 * m], vr[i][2 * m + 1]);
-            }
+    // piece j of 4 C of what this thread converts: eight codes
+    auto convert = [&](int b, int j) {
+        const int i = j / 4, m = j % 2;
+        const u4 x = j / 2 % 2 ? vr[i] : kr[i];
+        image[b][j / 2 % 2][((w + 4 * i) * 2 + m) * 64 + lane] = to_half<FMT>(x[2 * m], x[2 * m + 1]);
     };
     Lane ln = load(mine.lo), next{};
     Sight sight[N];
@@ -817,7 +817,8 @@ prompt_kernel(Args a, int32_t heads)
         sight[n] = sight_of(view, col[n]);
         st[n].init();
     }
-    convert(0);
+#pragma unroll
+    for (int j = 0; j < 4 * C; ++j) convert(0, j);
     next = load(mine.lo + 1);
     __syncthreads();
     // tile t, in buffer B (a constant: reads of one buffer and writes of the other may then pass each other)
@@ -825,27 +826,26 @@ prompt_kernel(Args a, int32_t heads)
         constexpr int b = decltype(buffer)::value;
         f4 s[N][4];
         {
+            // Fragment i: key rows q = i / (2 C), dimensions (k, m).  Left alone, the compiler reads a fragment, waits
+            // for it and multiplies; here the order is fixed: a read three fragments ahead, the products of this one,
+            // and at every second a piece of the next tile's conversion (past the last tile: of what was there, for
+            // nobody), which the vector units do beside them.
             const h8 *x = &image[b][0][lane];
+            h8 f[FR];
 #pragma unroll
-            for (int i = 0; i < FR; ++i) {   // fragment i: key rows q = i / (2 C), dimensions (k, m)
-                const int q = i / (2 * C), k = i / 2 % C, m = i % 2;
-                const h8 f = x[i * 64];
-#pragma unroll
-                for (int n = 0; n < N; ++n) s[n][q] = mfma(f, qh[n][k][m], i % (2 * C) ? s[n][q] : f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int n = 0; n < N; ++n) s[n][q] = mfma(f, ql[n][k][m], s[n][q]);
-            }
-            // Left alone, the compiler reads a fragment, waits for it and multiplies: 306 us where reading three ahead
-            // takes 283 (four prompts of 363 to 3690 tokens, 32 heads over 8, e4m3).
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+            for (int i = 0; i < 3; ++i) f[i] = x[i * 64];
 #pragma unroll
             for (int i = 0; i < FR; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 2 * N, 0);
-                if (i + 3 < FR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                const int q = i / (2 * C), k = i / 2 % C, m = i % 2;
+                if (i + 3 < FR) f[i + 3] = x[(i + 3) * 64];
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n][q] = mfma(f[i], qh[n][k][m], i % (2 * C) ? s[n][q] : f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n][q] = mfma(f[i], ql[n][k][m], s[n][q]);
+                if (i % 2) convert(b ^ 1, i / 2);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        convert(b ^ 1);   // of tile t + 1; past the last tile, of what was there, for nobody
         const Lane here = ln;
         ln = next;
         next = load(t + 2);
@@ -915,57 +915,82 @@ prompt_kernel(Args a, int32_t heads)
 }
 
 // ---------------------------------------------------------------- join the parts
-// Workgroup (head fastest): 16 rows of one row tile that was split; thread (row,
-// 16 lanes) takes D / 16 of a row's floats.  Four parts' loads are in flight at a time.
+// Workgroup (head fastest): 16 rows of one row tile that was split.  A unit is
+// four floats of a row; where the tile has fewer than 256 of them (few rows, as in
+// a decode step), the parts are dealt out to slices of the threads, whose sums
+// are added through LDS, in the order of the slices.
 template <int D, int R>
 __global__ void __launch_bounds__(256)
 join_kernel(Args a, int32_t heads)
 {
+    constexpr int Q = D / 4;   // units of a row
+    __shared__ f4 xs[256];
+    __shared__ float ms[256], ls[256];
     const int tid = threadIdx.x;
     const int32_t kvh = blockIdx.x % heads, sub = blockIdx.x / heads % (R / 16);
     const Item it = find_item<R>(a, blockIdx.x / heads / (R / 16), heads, true);
     if (!it.ok || it.n_split == 1 || (it.part + it.n_split - 1) * heads + kvh >= a.n_part) return;
+    const int32_t left = it.q.n * a.group - (it.tile * R + 16 * sub);   // rows from the first of these on
+    if (left <= 0) return;
     const Range all = tile_keys<R>(a, it, view_of(a, it));
     const int32_t n = all.hi - all.lo, per = (n + it.n_split - 1) / it.n_split;
     const int32_t parts = per ? (n + per - 1) / per : 0;   // the others are empty
-    const int row = 16 * sub + (tid >> 4);
-    const Place out = row_of(a, it, kvh, (uint32_t)it.tile * R, row);
-    if (out.token < 0) return;
-    auto index = [&](int32_t p) { return (int64_t)((it.part + min(p, parts - 1)) * heads + kvh) * R + row; };
-    float m = -INFINITY;
-    for (int32_t p = 0; p < parts; p += 16) m = fmaxf(m, a.part_ml[index(p + (tid & 15)) * 2]);
+    int rows = 1;                                          // a power of two that holds the rows
+    while (rows < min(left, 16)) rows *= 2;
+    const int units = rows * Q, slices = max(1, 256 / units);
+    for (int u0 = 0; u0 < units; u0 += 256) {
+        const int u = u0 + tid % min(units, 256), slice = tid / min(units, 256);
+        const int row = 16 * sub + u / Q, d = 4 * (u % Q);
+        auto index = [&](int32_t p) { return (int64_t)((it.part + p) * heads + kvh) * R + row; };
+        float m = -INFINITY, sum = 0.f;
+        f4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int32_t p0 = slice; p0 < parts; p0 += 8 * slices) {
+            f4 y[8];
+            float ym[8], yl[8], top = m;
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    f4 x[D / 64];
+            for (int i = 0; i < 8; ++i) {
+                const int32_t p = p0 + i * slices;
+                const int64_t at = index(p < parts ? p : p0);
+                ym[i] = a.part_ml[at * 2];
+                yl[i] = p < parts ? a.part_ml[at * 2 + 1] : 0.f;
+                y[i] = *reinterpret_cast<const f4 *>(a.part + at * D + d);
+                top = fmaxf(top, ym[i]);
+            }
+            sum = times2(sum, m - top);
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) x[d] = f4{0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    for (int32_t p = 0; p < parts; p += 4) {
-        f4 y[4][D / 64];
-        float ym[4], yl[4];
+            for (int e = 0; e < 4; ++e) x[e] = times2(x[e], m - top);
+            m = top;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t at = index(p + i);
-            ym[i] = a.part_ml[at * 2];
-            yl[i] = a.part_ml[at * 2 + 1];
+            for (int i = 0; i < 8; ++i) {
+                sum += times2(yl[i], ym[i] - m);
+                if (p0 + i * slices < parts)
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-                y[i][d] = *reinterpret_cast<const f4 *>(a.part + at * D + 64 * d + 4 * (tid & 15));
+                    for (int e = 0; e < 4; ++e) x[e] += times2(y[i][e], ym[i] - m);
+            }
         }
+        if (slices > 1) {
+            xs[tid] = x;
+            ms[tid] = m;
+            ls[tid] = sum;
+            __syncthreads();
+            if (slice) return;   // units <= 128: the loop ends here
+            for (int i = 1; i < slices; ++i) m = fmaxf(m, ms[u + i * units]);
+            x = f4{0.f, 0.f, 0.f, 0.f};
+            sum = 0.f;
+            for (int i = 0; i < slices; ++i) {
+                const int at = u + i * units;
+                const float d2 = ms[at] - m;
+                const f4 y = xs[at];
+                sum += times2(ls[at], d2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (p + i >= parts) break;
-            sum += times2(yl[i], ym[i] - m);
-#pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) x[d][u] += times2(y[i][d][u], ym[i] - m);
+                for (int e = 0; e < 4; ++e) x[e] += times2(y[e], d2);
+            }
         }
+        const Place out = row_of(a, it, kvh, (uint32_t)it.tile * R, row);
+        if (out.token < 0) continue;
+        const float div = sum != 0.f ? 0x1p-15f / sum : 0.f;
+        *reinterpret_cast<f4 *>(a.O + (int64_t)out.token * a.ldo + out.head * D + d) = x * div;
     }
-    const float div = sum != 0.f ? 0x1p-15f / sum : 0.f;
-    float *to = a.O + (int64_t)out.token * a.ldo + out.head * D + 4 * (tid & 15);
-#pragma unroll
-    for (int d = 0; d < D / 64; ++d) *reinterpret_cast<f4 *>(to + 64 * d) = x[d] * div;
 }
 
 // ---------------------------------------------------------------- how a call is split
@@ -982,22 +1007,30 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
 {
     const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256, heads = kv->n_kv_heads, group = n_heads / heads;
     Plan p{};
-    const bool few = rows * group <= 32 * (int64_t)n_seqs;
-    const bool wide = kv->head_dim < 256 && rows * group * heads >= 128 * cus;
+    const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
+    // The tile of a request's rows by the work, in key tiles a CU (bounds: the lengths are on the device).  Rates of a
+    // full device rise with the rows a converted key tile serves, but larger tiles are fewer, and take longer each.  us,
+    // 32 heads over 8, D = 128, int8, tiles of 16 / 64 rows: 64 tokens after 4000: 24.1 / 27.3 (32 key tiles of 16 rows a
+    // CU), 16 prompts of 40: 22.4 / 11.4, 300 after 2000: 47.2 / 39.7 (84), 4 prompts of 300: 39.2 / 21.7, 32 after 2000:
+    // 16.8 / 18.3 (8), 16 requests of 8 after 1000: 13.3 / 27.0.  Of 64 / 128 rows: prompt of 1024: 35.6 / 45.2 (16 key tiles
+    // of 128 rows), 100 after 8000: 45.9 / 48.5 (16), prompt of 2048: 90.1 / 90.7 (64), of 4096: 284 / 260 (256), 200 after
+    // 16000: 170 / 118 (55).
+    auto tiles_of = [&](int r) { return std::min<int64_t>(n_seqs, rows) + rows * group / r; };
+    const bool few = rows * group <= 16 * (int64_t)n_seqs || tiles_of(16) * heads * most_keys < 16 * cus;
+    const bool wide = kv->head_dim < 256 && tiles_of(128) * heads * most_keys >= 48 * cus;
     p.rows = few ? 16 : wide ? 128 : 64;
     p.least = 4;
-    p.target = few ? (kv->head_dim == 256 ? 1 : kv->head_dim == 128 ? 4 : 2) * cus : (kv->head_dim == 256 ? 1 : 2) * cus;
-    if (getenv("T_ROWS")) p.rows = atoi(getenv("T_ROWS"));
-    if (getenv("T_TARGET")) p.target = atoi(getenv("T_TARGET"));
-    if (getenv("T_LEAST")) p.least = atoi(getenv("T_LEAST"));
-    const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
-    p.tiles = std::min<int64_t>(n_seqs, rows) + rows * group / p.rows;   // sum of ceil(n_s group / R) over the n_s > 0
+    // The workgroups that a CU holds: at D = 256 the registers (16 rows) or LDS (64) allow one, else two.  One token each
+    // of 16 requests of 1033 to 4884 tokens, D = 256: 48.1 us with one wanted a CU, 50.1 with two, 67 with four; one
+    // request of 30000 tokens, D = 128: 22.4 with two, 28.4 with four.
+    p.target = (kv->head_dim == 256 ? 1 : 2) * cus;
+    p.tiles = tiles_of(p.rows);   // sum of ceil(n_s group / R) over the n_s > 0
     // up to 16 tiles a row tile's own workgroup does them in less time than a second launch takes
     const int64_t most_split = most_keys <= kWhole ? 1 : (most_keys + p.least - 1) / p.least;
-    // tiles * ceil(keys / length) <= tiles + work / length and work / length <= target / heads, summed in floats
-    p.items = std::min(p.tiles * most_split, p.tiles + p.target / heads + 2);
+    // tiles * ceil(keys / length) <= tiles + work / length and work / length <= 2 target / heads, summed in floats
+    p.items = std::min(p.tiles * most_split, p.tiles + 2 * p.target / heads + 2);
     // a tile that is split has more keys than one part, so its parts are at most twice its keys over the length
-    p.parts = most_split <= 1 ? 0 : std::min(p.items * heads, 2 * p.target + 4 * heads);
+    p.parts = most_split <= 1 ? 0 : std::min(p.items * heads, 4 * p.target + 4 * heads);
     return p;
 }
 
@@ -1061,6 +1094,15 @@ int64_t aih_kv_attention_scratch_floats(aih_ctx *ctx, const aih_kv_cache *kv, in
     if (rc) return rc;
     const Plan p = plan_of(ctx, kv, n_heads, rows, n_seqs, table_width);
     return ml_floats(p) + p.parts * p.rows * kv->head_dim;
+}
+
+int aih_kv_attention_tile_rows(aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs,
+                               int32_t table_width)
+{
+    if (!ctx) return AIH_E_INVALID;
+    int rc = aih_kv::check_shape(kv);
+    if (!rc) rc = check_batch(kv, n_heads, rows, n_seqs, table_width);
+    return rc ? rc : plan_of(ctx, kv, n_heads, rows, n_seqs, table_width).rows;
 }
 
 int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64_t ldq, float *O, int64_t ldo,

@@ -651,6 +651,12 @@ typedef struct aih_kv_scores {
  * n_seqs at most 4096, n_heads a multiple of n_kv_heads; scores may be NULL. */
 int64_t aih_kv_attention_scratch_floats(aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows,
                                         int32_t n_seqs, int32_t table_width);
+/* The rows ((token, head of the group) pairs of one KV head) per workgroup tile
+ * that such a call works on: 16, 64 or 128, by `rows`, n_seqs and table_width
+ * alone; or a negative status.  It lets tests and tools see which kernel a
+ * batch reaches. */
+int aih_kv_attention_tile_rows(aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs,
+                               int32_t table_width);
 int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64_t ldq, float *O, int64_t ldo,
                      int64_t rows, int32_t n_heads, int32_t n_seqs, const int32_t *starts, const int32_t *lens,
                      const int32_t *tables, int32_t table_width, float scale, const aih_kv_scores *scores,

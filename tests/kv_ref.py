@@ -141,15 +141,17 @@ class Cache:
 
 
 # ---- attention ---------------------------------------------------------------------
-def attention(cache, q, starts, lens, tables, scale, cap=0.0, window=0, slopes=None, prefix=None):
-    """q: (rows, n_heads, dim).  Returns (o, bound): the result and, for every
+def attention(cache, q, starts, lens, tables, scale, cap=0.0, window=0, slopes=None, prefix=None,
+              rows=None):
+    """q: (rows, n_heads, dim); rows: the ones wanted, None for all.  Returns (o, bound): the result and, for every
     row and head, what an fp32 evaluation may be off by (see `bound` below);
     rows of no request are NaN in both."""
-    rows, n_heads, dim = q.shape
+    n_rows, n_heads, dim = q.shape
+    wanted = set(range(n_rows) if rows is None else map(int, rows))
     kv, group = cache.heads, n_heads // cache.heads
     keys, vals = cache.values()
-    o = np.full((rows, n_heads, dim), np.nan)
-    bound = np.full((rows, n_heads), np.nan)
+    o = np.full((n_rows, n_heads, dim), np.nan)
+    bound = np.full((n_rows, n_heads), np.nan)
     q = q.astype(np.float64)
     for s in range(len(lens)):
         n, length = starts[s + 1] - starts[s], int(lens[s])
@@ -159,6 +161,8 @@ def attention(cache, q, starts, lens, tables, scale, cap=0.0, window=0, slopes=N
         slot = np.where(there, ids * cache.block + j % cache.block, 0)
         for i in range(n):
             p, r = length - n + i, starts[s] + i
+            if r not in wanted:
+                continue
             end = p + 1 if prefix is None else max(p + 1, int(prefix[s]))
             seen = there & (j < end)
             if window:

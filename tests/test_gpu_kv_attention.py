@@ -46,7 +46,7 @@ class Batch:
         self.q = (q_size * rng.standard_normal((self.rows, heads, dim))).astype(np.float32)
         self.scale = float(np.float32(1 / np.sqrt(dim)))
 
-    def run(self, cap=0.0, window=0, slopes=None, prefix=None, out=None, times=1, graph=False):
+    def run(self, cap=0.0, window=0, slopes=None, prefix=None, times=1):
         L, h = nat.lib(), self.dev.handle
         k, v = self.ref.packed()
         bufs = [upload(self.dev, k), upload(self.dev, v)] + [upload(self.dev, s.astype(np.float32)) for s in self.ref.scales]
@@ -79,6 +79,13 @@ class Batch:
             b.dispose()
         assert np.all(got[:, wide:] == -7)
         return got[:, :wide].reshape(self.rows, self.heads, self.dim)
+
+    def tile_rows(self):
+        """Rows per tile of the kernel that a call takes (aih_kv_attention_tile_rows)."""
+        c = nat.KvCache(format=self.ref.fmt, n_kv_heads=self.ref.heads, head_dim=self.dim, block_tokens=self.ref.block,
+                        n_blocks=self.ref.n_blocks)
+        return nat.lib().aih_kv_attention_tile_rows(self.dev.handle, ctypes.byref(c), self.heads, self.rows,
+                                                    len(self.lens), self.width)
 
     def check(self, bar=BAR, **kw):
         got = self.run(**kw)
@@ -136,6 +143,22 @@ def test_a_few_tokens(device, fmt, heads, kv, dim, block, lens, new):
     (8, 8, 128, 16, [130], [130]), (4, 1, 128, 64, [2500], [70]), (32, 1, 64, 16, [60], [60])])
 def test_prompts(device, fmt, heads, kv, dim, block, lens, new):
     Batch(device, fmt, heads, kv, dim, block, lens, new, pad=8, behind=2).check()
+
+
+@pytest.mark.parametrize("fmt,heads,kv,dim,lens,new,scores", [
+    (R.INT8, 32, 8, 128, [1500, 900], [1500, 900], dict()), (R.E4M3, 24, 8, 64, [2100, 40], [2000, 40], dict()),
+    (R.E4M3, 48, 8, 128, [1700], [1600], dict(cap=20.0, prefix=[500], window=1000)),
+    (R.INT8, 8, 1, 64, [9000], [1500], dict(slopes=[0.01] * 8))])
+def test_large_prompts(device, fmt, heads, kv, dim, lens, new, scores):
+    """Enough work for tiles of 128 rows.  The oracle takes every 37th row."""
+    b = Batch(device, fmt, heads, kv, dim, 32, lens, new, q_size=4.0 if "cap" in scores else 1.0)
+    assert b.tile_rows() == 128
+    got = b.run(**scores)
+    rows = np.arange(0, int(b.starts[-1]), 37)
+    want, bound = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale, rows=rows, **scores)
+    assert within(got[rows], want[rows], bound[rows])
+    nrm = np.linalg.norm(got[rows] - want[rows]) / np.linalg.norm(want[rows])
+    assert nrm <= (4 * BAR if "cap" in scores else BAR), nrm
 
 
 SCORES = [dict(cap=30.0), dict(cap=2.0), dict(window=1), dict(window=17), dict(window=64, cap=50.0), dict(slopes=True),

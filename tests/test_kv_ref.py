@@ -157,11 +157,14 @@ def test_attention_refuses_caches():
                                   1 << 40) == want, kw
     for kw, want in SHAPES:
         assert L.aih_kv_attention_scratch_floats(CTX, ctypes.byref(cache(**kw)), 4, 8, 2, 4) == want, kw
+        assert L.aih_kv_attention_tile_rows(CTX, ctypes.byref(cache(**kw)), 4, 8, 2, 4) == want, kw
     ok = ctypes.byref(cache())
     assert L.aih_kv_attention_scratch_floats(None, ok, 4, 8, 2, 4) == INV
     assert L.aih_kv_attention_scratch_floats(CTX, None, 4, 8, 2, 4) == INV
     for bad in ((3, 8, 2, 4), (4, -1, 2, 4), (4, 8, 0, 4), (4, 8, 2, 0)):
         assert L.aih_kv_attention_scratch_floats(CTX, ok, *bad) == INV
+        assert L.aih_kv_attention_tile_rows(CTX, ok, *bad) == INV
+    assert L.aih_kv_attention_tile_rows(None, ok, 4, 8, 2, 4) == INV
     assert L.aih_kv_attention_scratch_floats(CTX, ok, 4, 8, 4097, 4) == LIM
     # tables too short to be split need no scratch; longer ones do
     assert L.aih_kv_attention_scratch_floats(CTX, ok, 4, 8, 2, 4) == 0
