@@ -64,4 +64,34 @@ static inline int log2_of(int v) { return 31 - __builtin_clz((unsigned)v); }
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
+// Sum, inclusive scans and maximum over the 64 lanes on the DPP path (a shuffle
+// goes through LDS, ten times the latency): within rows of 16, then row 0 into row 1
+// and 2 into 3 (row_bcast:15), then rows 0, 1 into 2, 3 (row_bcast:31).  A lane
+// that nothing is shifted into gets a zero.  `op` has to be associative, with 0 for its unit.
+template <typename T, typename Op>
+__device__ __forceinline__ T wave_scan(T v, Op op)
+{
+    const T zero = 0;
+    v = op(v, __builtin_amdgcn_update_dpp(zero, v, 0x111, 0xF, 0xF, true));   // row_shr:1
+    v = op(v, __builtin_amdgcn_update_dpp(zero, v, 0x112, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_update_dpp(zero, v, 0x114, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_update_dpp(zero, v, 0x118, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_update_dpp(zero, v, 0x142, 0xA, 0xF, false));
+    return op(v, __builtin_amdgcn_update_dpp(zero, v, 0x143, 0xC, 0xF, false));
+}
+__device__ __forceinline__ int32_t wave_scan(int32_t v)
+{
+    return wave_scan(v, [](int32_t a, int32_t b) { return a + b; });
+}
+__device__ __forceinline__ float wave_add(float v)
+{
+    v = wave_scan(v, [](float a, float b) { return a + b; });
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+    v = wave_scan(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 }  // namespace aih_kv

@@ -50,6 +50,8 @@ namespace {
 
 using aih_kv::f4;
 using aih_kv::u4;
+using aih_kv::wave_add;
+using aih_kv::wave_scan;
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -103,30 +105,6 @@ struct Item {
     Seq q;
     bool ok;
 };
-
-// Sum and inclusive scan over the 64 lanes on the DPP path (a shuffle goes
-// through LDS, ten times the latency): within rows of 16, then row 0 into row 1
-// and 2 into 3 (row_bcast:15), then rows 0, 1 into 2, 3 (row_bcast:31).
-__device__ __forceinline__ float wave_add(float v)
-{
-    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x111, 0xF, 0xF, true);   // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0.0f, v, 0x143, 0xC, 0xF, false);
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-}
-__device__ __forceinline__ int32_t wave_scan(int32_t v)
-{
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
 
 // A lane's request: its row tiles and the key tiles of the longest of them.
 struct Load {

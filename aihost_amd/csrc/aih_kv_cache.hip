@@ -16,6 +16,8 @@ namespace {
 using aih_kv::f4;
 using aih_kv::kMaxSeqs;
 using aih_kv::u4;
+using aih_kv::wave_max;
+using aih_kv::wave_scan;
 
 // ---------------------------------------------------------------- block tables and slot maps
 // Sums of counts that stop at kFull: the largest value they are compared with
@@ -25,37 +27,43 @@ constexpr uint32_t kFull = 0x7FFFFFFFu;
 
 __device__ __forceinline__ uint32_t add_full(uint32_t a, uint32_t b) { return min(a + b, kFull); }
 
-// Inclusive scan of v over the 1024 threads of a workgroup, and the total.
-// red: 17 words of LDS, free again after the next barrier that follows.
-__device__ __forceinline__ uint32_t scan_1024(uint32_t v, uint32_t *red, uint32_t &total)
+// Inclusive scans of v and u over the threads of a workgroup, and their totals.
+// red: two words of LDS a wave.
+__device__ __forceinline__ void scan_pair(uint32_t &v, uint32_t &u, uint32_t (*red)[16], uint32_t &v_total,
+                                          uint32_t &u_total)
 {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(v, d);
-        if (lane >= d) v = add_full(v, o);
-    }
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    v = wave_scan(v, add_full);
+    u = wave_scan(u, add_full);
     __syncthreads();   // the last use of red
-    if (lane == 63) red[w] = v;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (i == w) before = total;
-        total = add_full(total, red[i]);
+    if (lane == 63) {
+        red[0][w] = v;
+        red[1][w] = u;
     }
-    return add_full(v, before);
+    __syncthreads();
+    uint32_t v_before = 0, u_before = 0;
+    v_total = u_total = 0;
+    for (int i = 0; i < waves; ++i) {
+        if (i == w) {
+            v_before = v_total;
+            u_before = u_total;
+        }
+        v_total = add_full(v_total, red[0][i]);
+        u_total = add_full(u_total, red[1][i]);
+    }
+    v = add_full(v, v_before);
+    u = add_full(u, u_before);
 }
 
-// The request of row r: the last s with starts[s] <= r (starts ascending,
-// starts[n] > r >= starts[0] = 0).
-__device__ __forceinline__ int request_of(const int32_t *starts, int n, int32_t r)
+// The request of row r (or of block r): the last s with firsts[s] <= r, for
+// ascending firsts with firsts[0] <= r.
+template <typename T>
+__device__ __forceinline__ int request_of(const T *firsts, int n, T r)
 {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (starts[mid] <= r) lo = mid;
+        if (firsts[mid] <= r) lo = mid;
         else hi = mid - 1;
     }
     return lo;
@@ -69,111 +77,109 @@ struct PlanArgs {
     int32_t n_seqs, width, shift, n_blocks, rows;
 };
 
-// Slot and position of row r, from the finished plan.  starts may be LDS or global.
-__device__ __forceinline__ void place_row(const PlanArgs &a, const int32_t *starts, const int32_t *new_lens, int32_t r)
+__device__ __forceinline__ int32_t slot_of(const PlanArgs &a, int32_t id, int32_t pos)
 {
-    int32_t slot = -1, pos = -1;
-    if (r < starts[a.n_seqs]) {
-        const int s = request_of(starts, a.n_seqs, r);
-        pos = new_lens[s] - (starts[s + 1] - r);
-        const int32_t id = a.tables[(int64_t)s * a.width + (pos >> a.shift)];
-        if (id >= 0 && id < a.n_blocks) slot = (id << a.shift) + (pos & ((1 << a.shift) - 1));
-    }
-    a.slots[r] = slot;
-    a.positions[r] = pos;
+    return id >= 0 && id < a.n_blocks ? (id << a.shift) + (pos & ((1 << a.shift) - 1)) : -1;
 }
 
-// One workgroup: two rounds of scans over the requests (blocks needed and rows
-// asked for, then rows granted), the handed-out blocks, and, with `place`,
-// the rows.  Latency is all there is to it at the sizes of a decode step: 64
-// requests read 512 bytes.
+// One workgroup of up to 1024 threads: two rounds of scans over the requests
+// (blocks needed and rows asked for; rows and blocks granted), then, with
+// `place`, the rows: each finds its request by bisection, takes its block from the
+// table or, a new one, off the stack, and the first of a block writes the table's
+// entry, so nothing waits for what another thread stores.  Else the blocks alone, and
+// place_kernel the rows.  A decode step's plan reads 512 bytes for 64 requests: a launch and four
+// memory round trips (lens, stack or table, and the stores).
 __global__ void __launch_bounds__(1024)
 plan_kernel(PlanArgs a, int place)
 {
     __shared__ int32_t starts[kMaxSeqs + 1];
-    __shared__ uint32_t upto[kMaxSeqs];    // blocks handed out up to and with request s
-    __shared__ int32_t had[kMaxSeqs];      // its blocks before; its new length in the end
-    __shared__ uint32_t red[17];
+    __shared__ uint32_t blocks[kMaxSeqs];   // blocks handed out before request s
+    __shared__ int32_t old[kMaxSeqs];       // its length before
+    __shared__ uint32_t red[2][16];
     __shared__ int32_t n_refused;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, threads = blockDim.x;
     const int32_t bt = 1 << a.shift;
     const uint32_t n_free = (uint32_t)min(max(*a.n_free, 0), a.n_blocks);
     if (tid == 0) n_refused = 0;
     uint32_t need_before = 0, asked_before = 0, rows_before = 0, taken = 0;
-    for (int base = 0; base < a.n_seqs; base += 1024) {
+    for (int base = 0; base < a.n_seqs; base += threads) {
         const int s = base + tid;
         int32_t len = 0, n = 0;
-        bool ok = s < a.n_seqs;
-        if (ok) {
+        const bool is = s < a.n_seqs;
+        if (is) {
             len = a.lens[s];
             n = a.n_new[s];
         }
         const bool valid = len >= 0 && n >= 0 && (int64_t)len + n <= (int64_t)a.width << a.shift;
-        const int32_t blocks = valid ? (int32_t)(((int64_t)len + bt - 1) >> a.shift) : 0;
-        uint32_t need = valid ? (uint32_t)((((int64_t)len + n + bt - 1) >> a.shift) - blocks) : 0u;
-        uint32_t total;
-        const uint32_t need_upto = add_full(scan_1024(need, red, total), need_before);
-        need_before = add_full(need_before, total);
-        const uint32_t asked = add_full(scan_1024(valid ? (uint32_t)n : 0u, red, total), asked_before);
-        asked_before = add_full(asked_before, total);
-        const bool fits = n == 0 || ((need == 0 || need_upto <= n_free) && asked <= (uint32_t)a.rows);
-        if (ok && !(valid && fits)) atomicAdd(&n_refused, 1);
-        ok = ok && valid && fits;
-        if (!ok) {
-            n = 0;
-            need = 0;
-        }
-        // granted requests that need blocks come before refused ones that do, so their sums are exact
-        const uint32_t begin = add_full(scan_1024((uint32_t)n, red, total), rows_before) - (uint32_t)n;
-        rows_before = add_full(rows_before, total);
-        (void)scan_1024(need, red, total);
-        taken += total;
-        if (s < a.n_seqs) {
-            starts[s] = (int32_t)begin;
-            had[s] = blocks;
-            upto[s] = need ? need_upto : 0u;
+        uint32_t need = valid ? (uint32_t)((((int64_t)len + n + bt - 1) >> a.shift) - (((int64_t)len + bt - 1) >> a.shift)) : 0u;
+        uint32_t need_upto = need, asked = valid ? (uint32_t)n : 0u, need_total, asked_total;
+        scan_pair(need_upto, asked, red, need_total, asked_total);
+        need_upto = add_full(need_upto, need_before);
+        asked = add_full(asked, asked_before);
+        need_before = add_full(need_before, need_total);
+        asked_before = add_full(asked_before, asked_total);
+        const bool ok = valid && (n == 0 || ((need == 0 || need_upto <= n_free) && asked <= (uint32_t)a.rows));
+        if (is && !ok) atomicAdd(&n_refused, 1);
+        if (!ok || !is) n = need = 0;
+        // (granted requests that need blocks come before refused ones that do: these sums are exact)
+        uint32_t end = (uint32_t)n, blocks_upto = need, end_total, blocks_total;
+        scan_pair(end, blocks_upto, red, end_total, blocks_total);
+        if (is) {
+            starts[s] = (int32_t)(rows_before + end) - n;
+            blocks[s] = taken + blocks_upto - need;
+            old[s] = len;
             a.new_lens[s] = len + n;
+            a.starts[s] = starts[s];
         }
+        rows_before += end_total;
+        taken += blocks_total;
     }
-    if (tid == 0) starts[a.n_seqs] = (int32_t)rows_before;
+    if (tid == 0) starts[a.n_seqs] = a.starts[a.n_seqs] = (int32_t)rows_before;
     __syncthreads();
-    for (int s = tid; s <= a.n_seqs; s += 1024) a.starts[s] = starts[s];
     if (tid == 0) {
         *a.new_n_free = (int32_t)(n_free - taken);
         *a.refused = n_refused;
     }
-    // The blocks: request s takes upto[s] - need .. upto[s] - 1 of the order; need from the lengths.
-    for (int s0 = (tid >> 6) * 64; s0 < a.n_seqs; s0 += 1024) {
-        // one wave, 64 requests: lane l looks at request s0 + l, the wave writes each one's entries together
-        const int s = s0 + (tid & 63);
-        int32_t need = 0, first = 0, at = 0;
-        if (s < a.n_seqs && upto[s]) {
-            at = had[s];
-            need = (int32_t)(((int64_t)a.new_lens[s] + bt - 1) >> a.shift) - at;
-            first = (int32_t)upto[s] - need;
+    const int32_t top = (int32_t)n_free - 1;
+    if (!place) {
+        for (uint32_t j = tid; j < taken; j += threads) {
+            const int s = request_of(blocks, a.n_seqs, j);
+            const int32_t at = (int32_t)(((int64_t)old[s] + bt - 1) >> a.shift) + (int32_t)(j - blocks[s]);
+            a.tables[(int64_t)s * a.width + at] = a.free_blocks[top - (int32_t)j];
         }
-        unsigned long long some = __ballot(need > 0);
-        while (some) {
-            const int l = __builtin_ctzll(some);
-            some &= some - 1;
-            const int32_t k = __shfl(need, l), f = __shfl(first, l), t = __shfl(at, l);
-            int32_t *to = a.tables + (int64_t)(s0 + l) * a.width + t;
-            for (int j = tid & 63; j < k; j += 64) to[j] = a.free_blocks[(int32_t)n_free - 1 - (f + j)];
-        }
+        return;
     }
-    if (!place) return;
-    __syncthreads();
-    for (int s = tid; s < a.n_seqs; s += 1024) had[s] = a.new_lens[s];
-    __syncthreads();
-    for (int32_t r = tid; r < a.rows; r += 1024) place_row(a, starts, had, r);
+    for (int32_t r = tid; r < a.rows; r += threads) {
+        int32_t slot = -1, pos = -1;
+        if (r < (int32_t)rows_before) {
+            const int s = request_of(starts, a.n_seqs, r);
+            pos = old[s] + (r - starts[s]);
+            const int32_t b = pos >> a.shift, had = (int32_t)(((int64_t)old[s] + bt - 1) >> a.shift);
+            int32_t *entry = a.tables + (int64_t)s * a.width + b;
+            const int32_t id = *(b < had ? entry : a.free_blocks + (top - (int32_t)blocks[s] - (b - had)));
+            if (b >= had && (pos & (bt - 1)) == 0) *entry = id;
+            slot = slot_of(a, id, pos);
+        }
+        a.slots[r] = slot;
+        a.positions[r] = pos;
+    }
 }
 
 // The rows of a plan, where they are too many for its one workgroup.
 __global__ void __launch_bounds__(256)
 place_kernel(PlanArgs a)
 {
-    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256)
-        place_row(a, a.starts, a.new_lens, (int32_t)r);
+    const int32_t total = a.starts[a.n_seqs];
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256) {
+        int32_t slot = -1, pos = -1;
+        if (r < total) {
+            const int s = request_of(a.starts, a.n_seqs, (int32_t)r);
+            pos = a.new_lens[s] - (a.starts[s + 1] - (int32_t)r);
+            slot = slot_of(a, a.tables[(int64_t)s * a.width + (pos >> a.shift)], pos);
+        }
+        a.slots[r] = slot;
+        a.positions[r] = pos;
+    }
 }
 
 __global__ void __launch_bounds__(1024)
@@ -181,7 +187,7 @@ release_kernel(int32_t *lens, int32_t n_seqs, int32_t *tables, int32_t width, in
                const int32_t *done, int32_t *free_blocks, int32_t *n_free)
 {
     __shared__ uint32_t first[kMaxSeqs];   // a request's blocks; then where they go on the stack
-    __shared__ uint32_t red[17];
+    __shared__ uint32_t red[2][16];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const uint32_t had = (uint32_t)min(max(*n_free, 0), n_blocks);
     auto blocks_of = [&](int s) {
@@ -198,13 +204,14 @@ release_kernel(int32_t *lens, int32_t n_seqs, int32_t *tables, int32_t width, in
         if (lane == 0) first[s] = c;
     }
     __syncthreads();
-    uint32_t before = 0, total;
+    uint32_t before = 0;
     for (int base = 0; base < n_seqs; base += 1024) {
         const int s = base + tid;
         const uint32_t c = s < n_seqs ? first[s] : 0u;
-        const uint32_t up = add_full(scan_1024(c, red, total), before);
+        uint32_t up = c, none = 0, total, zero;
+        scan_pair(up, none, red, total, zero);
+        if (s < n_seqs) first[s] = add_full(up, before) - c;
         before = add_full(before, total);
-        if (s < n_seqs) first[s] = up - c;
     }
     __syncthreads();
     for (int s = w; s < n_seqs; s += 16) {
@@ -341,19 +348,58 @@ __device__ __forceinline__ Scale next_scale(uint32_t top, float old, bool fresh)
     }
     if (top != 0 && o.s == 0.0f) o.s = F::first_scale(amax);
     else if (top != 0) {
-        const double most = (double)F::kMost * (double)o.s;   // exact
-        if ((double)amax > most) {
-            // the smallest d with amax <= most 2^d: the quotient's exponent, less one where it is a power of two (a
-            // quotient of 24 by 31 bits that is none stays further from it than fp64 rounds)
-            const double q = (double)amax / most;
-            int e;
-            const double m = frexp(q, &e);
-            o.d = m > 0.5 ? e : e - 1;
-            o.s = ldexpf(o.s, o.d);
-        }
+        // the smallest d with amax <= most 2^d, from the fractions and exponents of the two (most is exact)
+        const double most = (double)F::kMost * (double)o.s;
+        const int d = __builtin_amdgcn_frexp_expf(amax) - __builtin_amdgcn_frexp_exp(most) +
+                      ((double)__builtin_amdgcn_frexp_mantf(amax) > __builtin_amdgcn_frexp_mant(most) ? 1 : 0);
+        o.d = max(d, 0);
+        o.s = ldexpf(o.s, o.d);
     }
     if (o.s != 0.0f) o.inv = 1.0f / o.s;
     return o;
+}
+
+// One token into a block, keys or values, by one wave: lane l holds dimensions
+// 4 l .. 4 l + 3 (x; lanes past the head's nothing).  codes, scale: the block's of
+// this head; o: the token's offset.
+template <int FMT, int D, bool KEYS>
+__device__ __forceinline__ void append_one(uint8_t *codes, float *scale, float old, const f4 x, int o, int bt)
+{
+    typedef Format<FMT> F;
+    constexpr int C = D / 64;
+    const int lane = threadIdx.x & 63;
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = max(top, __float_as_uint(x[u]) & 0x7FFFFFFFu);
+    const Scale s = next_scale<FMT>(wave_max(top), old, o == 0);
+    const bool bad = s.s != s.s;
+    if (lane == 0) *scale = s.s;
+    if (o == 0 || s.d) {   // the rest of the block: started anew, or rescaled
+        const float f = ldexpf(1.0f, -s.d);
+        for (int u = lane; u < bt * D / 16; u += 64) {
+            u4 *to = reinterpret_cast<u4 *>(codes) + u;
+            u4 w = {0u, 0u, 0u, 0u};
+            if (o) {
+                w = *to;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = F::shrink(w[i], f);
+            }
+            *to = w;
+        }
+        __threadfence_block();   // these stores before the token's, which go over them
+    }
+    if (4 * lane < D) {
+        const float xs[4] = {x[0], x[1], x[2], x[3]};
+        const uint32_t w = bad ? 0u : F::pack(xs, s.s, s.inv);
+        uint8_t *group = codes + (o >> 4) * 16 * D;
+        if constexpr (KEYS) {
+            const int d = 4 * lane, t = (o >> 2) & 3, r = o & 3;
+            *reinterpret_cast<uint32_t *>(group + (((t * C + d / 64) * 4 + r) * 4 + d % 64 / 16) * 16 + d % 16) = w;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) group[(4 * lane + u) * 16 + (o & 15)] = (uint8_t)(w >> (8 * u));
+        }
+    }
 }
 
 // Workgroup (x, y): KV head y and the runs of rows of one block that begin
@@ -361,9 +407,10 @@ __device__ __forceinline__ Scale next_scale(uint32_t top, float old, bool fresh)
 // those rows.  A run's values are read twice, for their largest magnitude and
 // to be rounded; the second time they come from the caches.  Every 16-byte
 // unit of the block belongs to one thread, which reads what it keeps of it
-// (rescaled where the scale grew) and writes it once.
+// (rescaled where the scale grew) and writes it once.  A run of one row, as in
+// a decode step, is done by two waves without LDS (append_one).
 template <int FMT, int D, bool ROPE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 append_kernel(AppendArgs a, int rpw)
 {
     typedef Format<FMT> F;
@@ -391,63 +438,76 @@ append_kernel(AppendArgs a, int rpw)
     }
     const int head = blockIdx.y, bt = 1 << a.shift;
     auto block_of = [&](int64_t r) {   // the block of row r, -1 for none
-        const int32_t slot = a.slots[r];
-        const int32_t b = slot < 0 ? -1 : slot >> a.shift;
+        const int32_t slot = a.slots[min(max(r, (int64_t)0), a.rows - 1)];
+        const int32_t b = slot < 0 || r < 0 || r >= a.rows ? -1 : slot >> a.shift;
         return b < a.n_blocks ? b : -1;
     };
-    // which of the rows r0 .. begin a run (rpw <= 64; the same in every wave)
-    bool begins = false;
-    if (lane < rpw && r0 + lane < a.rows) {
-        const int64_t r = r0 + lane;
-        const int32_t b = block_of(r);
-        begins = b >= 0 && (r == 0 || block_of(r - 1) != b);
-    }
-    unsigned long long runs = __ballot(begins);
+    // The blocks of rows r0 - 1 .. r0 + 62, the same in every wave: which of the rows r0 .. begin a run
+    // (rpw < 64), and how far the first ones reach.
+    const int32_t mine = block_of(r0 - 1 + lane), left = __shfl_up(mine, 1);
+    unsigned long long runs = __ballot(lane >= 1 && lane <= rpw && mine >= 0 && mine != left);
     while (runs) {
-        const int64_t r = r0 + __builtin_ctzll(runs);
+        const int first = __builtin_ctzll(runs);
         runs &= runs - 1;
-        const int32_t block = block_of(r);
+        const int64_t r = r0 - 1 + first;
+        const int32_t block = __builtin_amdgcn_readlane(mine, first);
         // the run: rows r .. r + n - 1
-        int64_t n = 1;
-        for (;;) {
-            const int64_t q = r + n + lane;
-            const unsigned long long other = __ballot(q >= a.rows || block_of(min(q, a.rows - 1)) != block);
-            if (other) {
-                n += __builtin_ctzll(other);
-                break;
-            }
-            n += 64;
+        const unsigned long long others = __ballot(lane > first && mine != block);
+        int64_t n = others ? __builtin_ctzll(others) - first : 64 - first;
+        while (!others) {
+            const unsigned long long more = __ballot(block_of(r + n + lane) != block);
+            n += more ? __builtin_ctzll(more) : 64;
+            if (more) break;
         }
         const int64_t at = (int64_t)block * a.heads + head;
         const float old_k = a.ks[at], old_v = a.vs[at];
-        __syncthreads();   // the LDS of the run before
-        row_of[tid] = -1;
-        __syncthreads();
-        for (int64_t j = tid; j < n; j += 256)
-            if (placed(r + j)) atomicMax(&row_of[a.slots[r + j] & (bt - 1)], (int32_t)min<int64_t>(j, 0x7FFFFFFF));
         const float *K = a.K + r * a.ldk + head * D, *V = a.V + r * a.ldv + head * D;
         auto key4 = [&](int64_t j, int d) {
             f4 x = *reinterpret_cast<const f4 *>(K + j * a.ldk + d);
             if constexpr (ROPE) x = rotate<D>(x, a.table, a.positions[r + j], d);
             return x;
         };
-        uint32_t tk = 0, tv = 0;
-        for (int64_t i = tid; i < n * NQ; i += 256) {
-            const int64_t j = i / NQ;
-            const int d = 4 * (int)(i % NQ);
-            if (!placed(r + j)) continue;
-            const f4 x = key4(j, d), y = *reinterpret_cast<const f4 *>(V + j * a.ldv + d);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                tk = max(tk, __float_as_uint(x[u]) & 0x7FFFFFFFu);
-                tv = max(tv, __float_as_uint(y[u]) & 0x7FFFFFFFu);
+        uint8_t *kb = a.k + at * bt * D, *vb = a.v + at * bt * D;
+        if (n == 1) {
+            const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+            if (w < 2 && placed(r)) {
+                const int o = __builtin_amdgcn_readfirstlane(a.slots[r]) & (bt - 1);
+                f4 x = {0.f, 0.f, 0.f, 0.f};
+                if (4 * lane < D) x = w ? *reinterpret_cast<const f4 *>(V + 4 * lane) : key4(0, 4 * lane);
+                if (w) append_one<FMT, D, false>(vb, a.vs + at, old_v, x, o, bt);
+                else append_one<FMT, D, true>(kb, a.ks + at, old_k, x, o, bt);
             }
+            continue;
         }
+        __syncthreads();   // the LDS of the run before
+        row_of[tid] = -1;
+        __syncthreads();
+        for (int64_t j = tid; j < n; j += 256)
+            if (placed(r + j)) atomicMax(&row_of[a.slots[r + j] & (bt - 1)], (int32_t)min<int64_t>(j, 0x7FFFFFFF));
+        // the largest magnitudes, two loads of each in flight
+        uint32_t tk = 0, tv = 0;
+        for (int64_t j0 = tid / NQ; j0 < n; j0 += 2 * (256 / NQ)) {
+            f4 x[2], y[2];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            tk = max(tk, (uint32_t)__shfl_xor(tk, d));
-            tv = max(tv, (uint32_t)__shfl_xor(tv, d));
+            for (int i = 0; i < 2; ++i) {
+                const int64_t j = j0 + i * (256 / NQ);
+                const int d = 4 * (tid % NQ);
+                x[i] = y[i] = f4{0.f, 0.f, 0.f, 0.f};
+                if (j < n && placed(r + j)) {
+                    x[i] = key4(j, d);
+                    y[i] = *reinterpret_cast<const f4 *>(V + j * a.ldv + d);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    tk = max(tk, __float_as_uint(x[i][u]) & 0x7FFFFFFFu);
+                    tv = max(tv, __float_as_uint(y[i][u]) & 0x7FFFFFFFu);
+                }
         }
+        tk = wave_max(tk);
+        tv = wave_max(tv);
         if (lane == 0) {
             top[0][tid >> 6] = tk;
             top[1][tid >> 6] = tv;
@@ -461,57 +521,52 @@ append_kernel(AppendArgs a, int rpw)
         if (tid == 64) a.vs[at] = sv.s;
         const bool bad_k = sk.s != sk.s, bad_v = sv.s != sv.s;
         const float fk = ldexpf(1.0f, -sk.d), fv = ldexpf(1.0f, -sv.d);
-        uint8_t *kb = a.k + at * bt * D, *vb = a.v + at * bt * D;
-        // keys: unit u holds 16 dimensions of one token
         for (int u = tid; u < bt * D / 16; u += 256) {
-            const int g = u & 3, rr = (u >> 2) & 3, c = (u >> 4) % C, t = (u >> 4) / C % 4, grp = u / D;
-            const int32_t j = row_of[16 * grp + 4 * t + rr];
-            u4 *to = reinterpret_cast<u4 *>(kb) + u;
-            u4 w = {0u, 0u, 0u, 0u};
-            if (j >= 0 && !bad_k) {
+            // key unit u: 16 dimensions of one token; value unit u: 16 tokens at one dimension.  What both need is
+            // loaded before either is rounded.
+            const int g = u & 3, rr = (u >> 2) & 3, c = (u >> 4) % C, t = (u >> 4) / C % 4, grp = u / D, d = u % D;
+            const int32_t jk = row_of[16 * grp + 4 * t + rr];
+            u4 *kt = reinterpret_cast<u4 *>(kb) + u, *vt = reinterpret_cast<u4 *>(vb) + u;
+            const bool new_k = jk >= 0 && !bad_k, keep_k = jk < 0 && !fresh;   // round it; leave or rescale it
+            uint32_t new_v = 0;                                                // bit i: token i is new
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f4 x = key4(j, 64 * c + 16 * g + 4 * i);
-                    const float xs[4] = {x[0], x[1], x[2], x[3]};
-                    w[i] = F::pack(xs, sk.s, sk.inv);
-                }
-            } else if (j < 0 && !fresh) {
-                if (sk.d == 0) continue;
-                w = *to;
+            for (int i = 0; i < 16; ++i) new_v |= row_of[16 * grp + i] >= 0 ? 1u << i : 0u;
+            const bool keep_v = !fresh && new_v != 0xFFFFu;
+            u4 wk = {0u, 0u, 0u, 0u}, wv = {0u, 0u, 0u, 0u};
+            if (keep_k && sk.d) {
+                wk = *kt;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = F::shrink(w[i], fk);
+                for (int i = 0; i < 4; ++i) wk[i] = F::shrink(wk[i], fk);
             }
-            *to = w;
-        }
-        // values: unit u holds 16 tokens at one dimension
-        for (int u = tid; u < bt * D / 16; u += 256) {
-            const int grp = u / D, d = u % D;
-            u4 *to = reinterpret_cast<u4 *>(vb) + u;
-            uint32_t fresh_bytes = 0;   // bit i: token i is new
-#pragma unroll
-            for (int i = 0; i < 16; ++i) fresh_bytes |= row_of[16 * grp + i] >= 0 ? 1u << i : 0u;
-            if (fresh_bytes == 0 && !fresh && sv.d == 0) continue;
-            u4 w = {0u, 0u, 0u, 0u};
-            if (!fresh && fresh_bytes != 0xFFFFu) {
-                w = *to;
+            if (keep_v && (new_v || sv.d)) {
+                wv = *vt;
                 if (sv.d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = F::shrink(w[i], fv);
+                    for (int i = 0; i < 4; ++i) wv[i] = F::shrink(wv[i], fv);
             }
+            // a word of either at a time: five loads in flight, few registers (with all twenty 167, and a third of the waves)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (!(fresh_bytes >> (4 * i) & 15)) continue;
-                float x[4];
+                f4 x = {0.f, 0.f, 0.f, 0.f};
+                float y[4];
                 uint32_t keep = 0;
+                if (new_k) x = key4(jk, 64 * c + 16 * g + 4 * i);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const int32_t j = row_of[16 * grp + 4 * i + b];
-                    x[b] = j >= 0 && !bad_v ? V[j * a.ldv + d] : 0.0f;
+                    y[b] = 0.f;
                     if (j < 0) keep |= 0xFFu << (8 * b);
+                    else if (!bad_v) y[b] = V[(int64_t)j * a.ldv + d];
                 }
-                w[i] = (w[i] & keep) | (F::pack(x, sv.s, sv.inv) & ~keep);
+                if (new_k) {
+                    const float xs[4] = {x[0], x[1], x[2], x[3]};
+                    wk[i] = F::pack(xs, sk.s, sk.inv);
+                }
+                if (keep != 0xFFFFFFFFu) wv[i] = (wv[i] & keep) | (F::pack(y, sv.s, sv.inv) & ~keep);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            *to = w;
+            if (!keep_k || sk.d) *kt = wk;
+            if (new_v || !keep_v || sv.d) *vt = wv;
         }
     }
 }
@@ -558,7 +613,8 @@ read_kernel(const uint8_t *__restrict__ k, const uint8_t *__restrict__ v, const 
 // placed by a second launch over the whole device.
 constexpr int64_t kPlaceRows = 4096;
 // Up to this many rows every workgroup of an append looks at one row, above
-// at 16: a prompt's rows come in runs, and a run is the work of its first row.
+// at a block's worth, at most 32: a prompt's rows come in runs, and a run is the
+// work of its first row.
 constexpr int64_t kSingleRows = 2048;
 
 template <int FMT, int D>
@@ -586,7 +642,7 @@ int append(aih_ctx *ctx, const aih_kv_cache *kv, AppendArgs a, bool rope)
     a.shift = aih_kv::log2_of(kv->block_tokens);
     a.q_parts = rope ? (int32_t)std::min<int64_t>(8, ((int64_t)a.q_heads * kv->head_dim + 1023) / 1024) : 0;
     if (a.heads + a.q_parts > 65535) return AIH_E_LIMIT;
-    const int rpw = a.rows <= kSingleRows ? 1 : 16;
+    const int rpw = a.rows <= kSingleRows ? 1 : std::min(kv->block_tokens, 32);
     aih_kv::DeviceGuard guard(ctx->device);
     AIH_TRY(guard.status);
     const bool i8 = kv->format == AIH_KV_INT8;
@@ -637,7 +693,9 @@ int aih_kv_plan(aih_ctx *ctx, const int32_t *lens, const int32_t *n_new, int32_t
     PlanArgs a{lens, n_new, tables, free_blocks, n_free, new_lens, new_n_free, starts, slots, positions, refused,
                n_seqs, table_width, aih_kv::log2_of(block_tokens), n_blocks, (int32_t)rows};
     const bool alone = rows <= kPlaceRows;
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, ctx->stream, a, alone ? 1 : 0);
+    // a wave for 64 requests or rows: barriers of few waves are short
+    const int64_t threads = std::min<int64_t>(1024, (std::max<int64_t>(n_seqs, alone ? rows : 1024) + 63) / 64 * 64);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3((unsigned)threads), 0, ctx->stream, a, alone ? 1 : 0);
     if (!alone) {
         const int rc = aih_launch_status();
         if (rc) return rc;
