@@ -33,6 +33,7 @@ import numpy as np
 
 from . import _native as nat
 from .compute import HipComputeDevice, fill_normal, quantize, row_bytes  # noqa: F401
+from .kvcache import PagedKvCache
 
 Q4_K, Q6_K, F32 = nat.Q4_K, nat.Q6_K, nat.F32
 
@@ -204,9 +205,14 @@ class DeviceWeights:
 
 
 class LlamaDecoder:
-    """Prefill + greedy decode of one sequence of up to max_len positions."""
+    """Prefill + greedy decode of one sequence of up to max_len positions.
 
-    def __init__(self, device, cfg, weights, max_len, max_prefill):
+    kv_format: None keeps the keys and values in fp32 (rows of max_len
+    positions per layer); "int8" or "e4m3" in a paged cache of 8-bit codes
+    with a scale per block and head (PagedKvCache), a quarter of the bytes
+    that a decode step reads of them."""
+
+    def __init__(self, device, cfg, weights, max_len, max_prefill, kv_format=None):
         if cfg.head_dim != 128:
             raise ValueError("the attention kernels need head_dim 128")
         if max_prefill > max_len:
@@ -240,8 +246,16 @@ class LlamaDecoder:
         self.qkv = buf(P * (qd + 2 * c.kv_dim) * 4)
         self.gu = buf(c.ffn * 4)
         self.logits = buf(c.vocab * 4)
-        self.kc = [buf(self.max_len * c.kv_dim * 4) for _ in range(c.n_layers)]
-        self.vc = [buf(self.max_len * c.kv_dim * 4) for _ in range(c.n_layers)]
+        self.paged = None
+        if kv_format is not None:
+            block = 32
+            self.paged = PagedKvCache(device, c.n_layers, c.n_kv_heads, c.head_dim, -(-self.max_len // block), 1,
+                                      self.max_len, P, kv_format, block)
+            for rows in {1, P}:
+                self.paged.reserve(c.n_heads, rows)
+        cached = c.n_layers if kv_format is None else 0
+        self.kc = [buf(self.max_len * c.kv_dim * 4) for _ in range(cached)]
+        self.vc = [buf(self.max_len * c.kv_dim * 4) for _ in range(cached)]
         self.scratch_floats = int(self.L.aih_attention_scratch_floats(c.n_heads, self.max_len))
         nat.check(self.scratch_floats if self.scratch_floats < 0 else 0, "aih_attention_scratch_floats")
         self.scratch = buf(self.scratch_floats * 4)
@@ -308,6 +322,14 @@ class LlamaDecoder:
         c, L, h, p = self.cfg, self.L, self.h, "blk.%d." % l
         qd = c.n_heads * c.head_dim
         ld = qd + 2 * c.kv_dim
+        if self.paged is not None:
+            # the projection's rows, then rotation and the 8-bit store in one launch, then attention over the codes
+            self._mmx(p + "attn_qkv", self.x, self.w.ptr(p + "attn_norm"), nat.PRE_RMSNORM, nat.POST_STORE, rows,
+                      self.qkv)
+            self._paged_attention(l, self.qkv, ld, self.qkv + qd * 4, ld, self.qkv + (qd + c.kv_dim) * 4, ld)
+            self._mmx(p + "attn_output", self.att, None, nat.PRE_NONE, nat.POST_ACCUMULATE, rows, self.x)
+            self._ffn_fused(p, rows)
+            return
         # the Q|K|V GEMM with RoPE and the cache store in its epilogue (aih_qgemm_fused + aih_rope_qkv)
         qt, wp, n, k = self.w[p + "attn_qkv"]
         assert n == ld
@@ -320,6 +342,18 @@ class LlamaDecoder:
                                           c.n_kv_heads, c.head_dim, start, pos, self.max_len, self.scale),
                   "attention")
         self._mmx(p + "attn_output", self.att16, None, nat.PRE_F16_OPERAND, nat.POST_ACCUMULATE, rows, self.x)
+        self._ffn_fused(p, rows)
+
+    def _paged_attention(self, l, q, ldq, k, ldk, v, ldv):
+        """Rotation of q and k, the rows into layer l's paged cache, and the
+        attention of the step's rows over it, into self.att."""
+        c = self.cfg
+        self.paged.append_rope(l, q, ldq, c.n_heads, k, ldk, v, ldv, self.table, self.max_len)
+        self.paged.attention(l, q, ldq, self.att, c.n_heads * c.head_dim, c.n_heads, self.scale)
+
+    def _ffn_fused(self, p, rows):
+        """The feed-forward half of _prefill_layer_fused."""
+        c = self.cfg
         norm = self.w.ptr(p + "ffn_norm")
         if p + "ffn_gate_up" in self.w and (2 * c.ffn) % 128 == 0:
             # SiLU(gate)*up leaves the gate|up GEMM as the down GEMM's fp16 operand
@@ -335,7 +369,8 @@ class LlamaDecoder:
 
     def layer(self, l, rows, start, pos):
         """One decoder layer over `rows` activation rows at positions start..
-        (+*pos when pos is a device pointer).  A single row (decode) runs as
+        (+*pos when pos is a device pointer; with a paged cache: the rows of
+        its last plan).  A single row (decode) runs as
         six kernels: Q|K|V matvec with the attention RMSNorm fused in,
         attention with RoPE and the KV cache store fused in (two kernels),
         W_o matvec adding into x, gate|up matvec with the FFN RMSNorm fused in
@@ -359,7 +394,10 @@ class LlamaDecoder:
             self._mm(p + "attn_k", self.xn, rows, self.k)
             self._mm(p + "attn_v", self.xn, rows, self.v)
             q, k, v = self.q, self.k, self.v
-        if decode and self.fused_attention:
+        if self.paged is not None:
+            ld = (qd + 2 * c.kv_dim) if decode else qd
+            self._paged_attention(l, q, ld, k, ld if decode else c.kv_dim, v, ld if decode else c.kv_dim)
+        elif decode and self.fused_attention:
             nat.check(L.aih_attention_decode_qkv(h, self.qkv, self.kc[l], self.vc[l], self.att, c.n_heads,
                                                  c.n_kv_heads, c.head_dim, start, pos, self.table, self.max_len,
                                                  self.max_len, self.scale, self.scratch, self.scratch_floats),
@@ -414,6 +452,10 @@ class LlamaDecoder:
         nat.check(self.L.aih_memcpy_h2d(self.h, self.ids, ids.ctypes.data, ids.nbytes), "ids")
         qt, tb, vocab, dim = self.w["token_embd"]
         nat.check(self.L.aih_embed_q(self.h, qt, tb, vocab, dim, self.ids, n, self.x), "embed")
+        if self.paged is not None:
+            self.paged.release()
+            self.paged.plan([n], n)
+            self.paged.set_new([1])      # for the decode steps that follow
         for l in range(c.n_layers):
             self.layer(l, n, 0, None)
         # decode bookkeeping: the first token is history[0]; position becomes n
@@ -431,6 +473,8 @@ class LlamaDecoder:
         c = self.cfg
         qt, tb, vocab, dim = self.w["token_embd"]
         nat.check(self.L.aih_embed_q(self.h, qt, tb, vocab, dim, self.token, 1, self.x), "embed")
+        if self.paged is not None:
+            self.paged.plan(rows=1)
         for l in range(c.n_layers):
             self.layer(l, 1, 0, self.pos)
         self.head(self.x, self.pos, self.n_prompt - 1)
@@ -499,6 +543,9 @@ class LlamaDecoder:
         if self.graph is not None:
             self.L.aih_graph_destroy(self.graph)
             self.graph = None
+        if self.paged is not None:
+            self.paged.dispose()
+            self.paged = None
         for b in self._bufs:
             b.dispose()
         self._bufs = []
