@@ -978,6 +978,7 @@ struct Plan {
     int64_t target, tiles, items, parts;   // bounds over one KV head (tiles, items) and over all (parts)
 };
 
+// Up to this many key tiles are not split: a row tile's own workgroup does them in less time than a second launch takes.
 constexpr int64_t kWhole = 16;
 
 Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs,
@@ -986,25 +987,32 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
     const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256, heads = kv->n_kv_heads, group = n_heads / heads;
     Plan p{};
     const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
-    // The tile of a request's rows by the work, in key tiles a CU (bounds: the lengths are on the device).  Rates of a
-    // full device rise with the rows a converted key tile serves, but larger tiles are fewer, and take longer each.  us,
-    // 32 heads over 8, D = 128, int8, tiles of 16 / 64 rows: 64 tokens after 4000: 24.1 / 27.3 (32 key tiles of 16 rows a
-    // CU), 16 prompts of 40: 22.4 / 11.4, 300 after 2000: 47.2 / 39.7 (84), 4 prompts of 300: 39.2 / 21.7, 32 after 2000:
-    // 16.8 / 18.3 (8), 16 requests of 8 after 1000: 13.3 / 27.0.  Of 64 / 128 rows: prompt of 1024: 35.6 / 45.2 (16 key tiles
-    // of 128 rows), 100 after 8000: 45.9 / 48.5 (16), prompt of 2048: 90.1 / 90.7 (64), of 4096: 284 / 260 (256), 200 after
-    // 16000: 170 / 118 (55).
     auto tiles_of = [&](int r) { return std::min<int64_t>(n_seqs, rows) + rows * group / r; };
-    const bool few = rows * group <= 16 * (int64_t)n_seqs || tiles_of(16) * heads * most_keys < 16 * cus;
-    const bool wide = kv->head_dim < 256 && tiles_of(128) * heads * most_keys >= 48 * cus;
-    p.rows = few ? 16 : wide ? 128 : 64;
+    // The tile of a request's rows, by what a call would take with requests of equal rows and full tables (the lengths
+    // are on the device).  Tiles of 16: 0.5 us of a CU for a tile and 64 keys, and 5 us for every further round of
+    // workgroups; of 64: 1.1 us, or 1.25 us one after the other for the keys of a part, and 12 us for a join.  Measured,
+    // 32 heads over 8, D = 128, int8, us of 16 / 64: 64 tokens after 4000 24.1 / 27.3, 100 after 8000 57.4 / 45.8, 300
+    // after 2000 47.2 / 39.7, 16 requests of 16 after 1000 20.6 / 28.3, of 8 after 1000 13.3 / 27.0, 4 prompts of 100
+    // 14.7 / 9.4, 16 of 40 22.4 / 11.4, one of 150 8.5 / 10.2, of 300 14.3 / 13.1, 8 of 32 after 500 15.1 / 19.4.
+    // Tiles of 128 use a converted key twice as often but are fewer and take longer each: us of 64 / 128: prompt of 1024
+    // 35.6 / 45.2 (16 tiles of 128 rows and 64 keys a CU), 100 after 8000 45.9 / 48.5 (16), prompt of 2048 90.1 / 90.7
+    // (64), of 4096 284 / 260 (256), 200 after 16000 170 / 118 (55).
+    const double per_seq = (double)(rows * group) / n_seqs, keys = (double)most_keys, cu = (double)cus;
+    auto groups_of = [&](int r) { return n_seqs * std::ceil(per_seq / r) * (double)heads; };
+    const bool joined = most_keys > kWhole;
+    const double g16 = groups_of(16), g64 = groups_of(64);
+    const double us16 = 5.0 * std::max(0.0, g16 / (2 * cu) - 1) + 0.5 * g16 * keys / cu;
+    const double part64 = joined ? std::max(4.0, keys * std::min(1.0, g64 / (2 * cu))) : keys;
+    const double us64 = std::max(1.25 * part64, 1.1 * g64 * keys / cu) + (joined ? 12.0 : 0.0);
+    const bool wide = kv->head_dim < 256 && (double)(tiles_of(128) * heads) * keys >= 48 * cu;
+    p.rows = us16 < us64 ? 16 : wide ? 128 : 64;
     p.least = 4;
     // The workgroups that a CU holds: at D = 256 the registers (16 rows) or LDS (64) allow one, else two.  One token each
     // of 16 requests of 1033 to 4884 tokens, D = 256: 48.1 us with one wanted a CU, 50.1 with two, 67 with four; one
     // request of 30000 tokens, D = 128: 22.4 with two, 28.4 with four.
     p.target = (kv->head_dim == 256 ? 1 : 2) * cus;
     p.tiles = tiles_of(p.rows);   // sum of ceil(n_s group / R) over the n_s > 0
-    // up to 16 tiles a row tile's own workgroup does them in less time than a second launch takes
-    const int64_t most_split = most_keys <= kWhole ? 1 : (most_keys + p.least - 1) / p.least;
+    const int64_t most_split = !joined ? 1 : (most_keys + p.least - 1) / p.least;
     // tiles * ceil(keys / length) <= tiles + work / length and work / length <= 2 target / heads, summed in floats
     p.items = std::min(p.tiles * most_split, p.tiles + 2 * p.target / heads + 2);
     // a tile that is split has more keys than one part, so its parts are at most twice its keys over the length
