@@ -439,6 +439,14 @@ struct QRow {
 // l-th: its place in the cache (in groups; kNone past the request's tokens or
 // outside the cache) and its scales.  In two steps, the table's entries and what
 // they lead to, so that a loop over tiles can take them ahead of their use.
+// What a lane reads in place of a group that is not there: a weight of 0 times a
+// byte that is no number would be none.
+__device__ const u4 no_group[256] = {};   // 16 tokens of 256 dimensions
+__device__ __forceinline__ const uint8_t *group_ptr(const uint8_t *codes, uint32_t at, int bytes)
+{
+    return at == kNone ? reinterpret_cast<const uint8_t *>(no_group) : codes + (size_t)at * bytes;
+}
+
 constexpr float kHidden = -1.0f;   // the value scale of a group that is not there
 struct Groups {
     uint32_t at;
@@ -626,7 +634,7 @@ few_kernel(Args a, int32_t heads)
     u4 kr[4][C], vr[DT];
     auto load_k = [&](int32_t t) {
         const uint32_t at = __shfl(walk.now.at, 4 * ((t - t0) & 15) + (c >> 2));
-        const uint8_t *kp = a.k + (size_t)(at == kNone ? 0 : at) * (16 * D) + ((c & 3) * 4 + g) * 16;
+        const uint8_t *kp = group_ptr(a.k, at, 16 * D) + ((c & 3) * 4 + g) * 16;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -635,7 +643,7 @@ few_kernel(Args a, int32_t heads)
     auto load_v = [&](int32_t t) {
         const int from = 4 * ((t - t0) & 15) + g;
         const uint32_t at = __shfl(walk.now.at, from);
-        const uint8_t *vp = a.v + (size_t)(at == kNone ? 0 : at) * (16 * D) + c * 16;
+        const uint8_t *vp = group_ptr(a.v, at, 16 * D) + c * 16;
 #pragma unroll
         for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const u4 *>(vp + d * 256);
         return Lane{__shfl(walk.now.ks, from), __shfl(walk.now.vs, from)};
@@ -767,8 +775,8 @@ prompt_kernel(Args a, int32_t heads)
         walk.advance(a, it, kvh, heads, mine.lo, mine.hi, t);
         const int in = (t - mine.lo) & 15;
         const uint32_t at_k = __shfl(walk.now.at, 4 * in + (c >> 2)), at_v = __shfl(walk.now.at, 4 * in + g);
-        const uint8_t *kp = a.k + (size_t)(at_k == kNone ? 0 : at_k) * (16 * D) + ((c & 3) * 4 + g) * 16 + w * 256;
-        const uint8_t *vp = a.v + (size_t)(at_v == kNone ? 0 : at_v) * (16 * D) + c * 16 + w * 256;
+        const uint8_t *kp = group_ptr(a.k, at_k, 16 * D) + ((c & 3) * 4 + g) * 16 + w * 256;
+        const uint8_t *vp = group_ptr(a.v, at_v, 16 * D) + c * 16 + w * 256;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             kr[i] = *reinterpret_cast<const u4 *>(kp + i * 1024);

@@ -300,3 +300,40 @@ def test_shape_of_the_batch_does_not_change_a_short_row(device):
         one.__dict__.update(b.__dict__)
         one.lens, one.tables, one.starts, one.rows, one.q = [b.lens[s]], b.tables[s:s + 1], np.array([0, 1]), 1, b.q[s:s + 1]
         np.testing.assert_array_equal(one.run()[0], both[s])
+
+
+@pytest.mark.parametrize("new", [[1, 1], [6, 2], [100, 70]])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_blocks_that_were_never_started(device, fmt, new):
+    """The pool as it comes: every block that no request holds full of bytes that are no number (0x7F, 0xFF), its scales
+    NaN.  The last tiles of these requests end inside such ground."""
+    b = Batch(device, fmt, 4, 2, 128, 16, [210, 75], new)
+    held = set(b.tables[b.tables >= 0].tolist())
+    assert len(held) < b.ref.n_blocks
+    # block 0, which hidden keys would be read from, is one that nobody holds
+    if 0 in held:
+        spare = next(x for x in range(b.ref.n_blocks) if x not in held)
+        b.ref.codes[:, [0, spare]] = b.ref.codes[:, [spare, 0]]
+        b.ref.scales[:, [0, spare]] = b.ref.scales[:, [spare, 0]]
+        b.tables[b.tables == 0] = spare
+        held = set(b.tables[b.tables >= 0].tolist())
+    plain = b.run()
+    empty = [x for x in range(b.ref.n_blocks) if x not in held]
+    b.ref.scales[:, empty] = np.nan
+    packed = b.ref.packed()
+    for a, byte in zip(packed, (0x7F, 0xFF)):
+        a.reshape(b.ref.n_blocks, -1)[empty] = byte
+    b.ref.packed = lambda: packed
+    np.testing.assert_array_equal(b.run(), plain)
+
+
+def test_many_requests_in_parts_and_prompts(device):
+    """More requests than the lanes of a wave: one of them long, so that it is split; prompts in tiles of 64 rows."""
+    lens = [5000 if s == 66 else 40 + s for s in range(80)]
+    b = Batch(device, R.INT8, 4, 1, 64, 32, lens, [1] * 80, seed=1)
+    assert b.tile_rows() == 16
+    b.check()
+    lens = [30 + s % 50 for s in range(130)]
+    b = Batch(device, R.E4M3, 8, 2, 64, 16, lens, lens, seed=2)
+    assert b.tile_rows() == 64
+    b.check()
