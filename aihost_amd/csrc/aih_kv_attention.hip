@@ -96,7 +96,7 @@ __device__ __forceinline__ int32_t row_tiles(const Args &a, const Seq &q)
 }
 __device__ __forceinline__ int32_t key_tiles(const Args &a, const Seq &q)
 {
-    const int32_t lo = a.window > 0 ? max(0, q.len - q.n + 1 - a.window) : 0;
+    const int32_t lo = a.window > 0 ? (int32_t)max<int64_t>(0, (int64_t)q.len - q.n + 1 - a.window) : 0;
     return (int32_t)(((int64_t)q.len + 63) / 64) - lo / 64;
 }
 
@@ -197,7 +197,10 @@ __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t he
 // min(max(p + 1, prefix), len) - 1.
 struct View {
     int32_t prefix, len, window;
-    __device__ __forceinline__ int32_t lo(int32_t p) const { return window > 0 ? max(0, p - window + 1) : 0; }
+    __device__ __forceinline__ int32_t lo(int32_t p) const
+    {
+        return window > 0 ? (int32_t)max<int64_t>(0, (int64_t)p - window + 1) : 0;
+    }
     __device__ __forceinline__ int32_t hi(int32_t p) const { return min(max(p + 1, prefix), len); }
 };
 
@@ -712,13 +715,14 @@ few_kernel(Args a, int32_t heads)
     for (int i = 0; i < 4; ++i) sum += times2(ls[i][row], ms[i][row] - m);
     const bool whole = it.n_split == 1;
     const Place out = row_of(a, it, kvh, (uint32_t)it.tile * 16, row);
-    const int32_t part = (it.part + it.split) * heads + kvh;
-    if (!whole && part >= a.n_part) return;   // never: the scratch is sized for every part
+    // starts in ascending order never have more parts than the scratch holds
+    const int64_t part = ((int64_t)it.part + it.split) * heads + kvh;
+    if (!whole && (it.part < 0 || part >= a.n_part)) return;
     const float div = !whole ? 1.0f : sum != 0.f ? 0x1p-15f / sum : 0.f;
-    float *to = whole ? a.O + (int64_t)out.token * a.ldo + out.head * D : a.part + ((int64_t)part * 16 + row) * D;
+    float *to = whole ? a.O + (int64_t)out.token * a.ldo + out.head * D : a.part + (part * 16 + row) * D;
     if (!whole && (tid & 15) == 0) {
-        a.part_ml[((int64_t)part * 16 + row) * 2] = m;
-        a.part_ml[((int64_t)part * 16 + row) * 2 + 1] = sum;
+        a.part_ml[(part * 16 + row) * 2] = m;
+        a.part_ml[(part * 16 + row) * 2 + 1] = sum;
     }
     if (out.token < 0) return;
 #pragma unroll
@@ -881,14 +885,15 @@ prompt_kernel(Args a, int32_t heads)
         if (t + 1 < mine.hi) step(std::integral_constant<int, 1>(), t + 1);
     }
     const bool whole = it.n_split == 1;
-    const int32_t part = (it.part + it.split) * heads + kvh;
-    if (!whole && part >= a.n_part) return;   // never: the scratch is sized for every part
+    // starts in ascending order never have more parts than the scratch holds
+    const int64_t part = ((int64_t)it.part + it.split) * heads + kvh;
+    if (!whole && (it.part < 0 || part >= a.n_part)) return;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const float sum = over4_sum(st[n].l);
         const Place out = row_of(a, it, kvh, (uint32_t)it.tile * R, 16 * N * w + 16 * n + c);
         if (out.token < 0) continue;
-        const int64_t row = (int64_t)part * R + 16 * N * w + 16 * n + c;
+        const int64_t row = part * R + 16 * N * w + 16 * n + c;
         float *to = whole ? a.O + (int64_t)out.token * a.ldo + out.head * D : a.part + row * D;
         if (!whole && g == 0) {
             a.part_ml[row * 2] = st[n].m;
@@ -915,7 +920,7 @@ join_kernel(Args a, int32_t heads)
     const int tid = threadIdx.x;
     const int32_t kvh = blockIdx.x % heads, sub = blockIdx.x / heads % (R / 16);
     const Item it = find_item<R>(a, blockIdx.x / heads / (R / 16), heads, true);
-    if (!it.ok || it.n_split == 1 || (it.part + it.n_split - 1) * heads + kvh >= a.n_part) return;
+    if (!it.ok || it.n_split == 1 || it.part < 0 || ((int64_t)it.part + it.n_split) * heads > a.n_part) return;
     const int32_t left = it.q.n * a.group - (it.tile * R + 16 * sub);   // rows from the first of these on
     if (left <= 0) return;
     const Range all = tile_keys<R>(a, it, view_of(a, it));
@@ -927,7 +932,7 @@ join_kernel(Args a, int32_t heads)
     for (int u0 = 0; u0 < units; u0 += 256) {
         const int u = u0 + tid % min(units, 256), slice = tid / min(units, 256);
         const int row = 16 * sub + u / Q, d = 4 * (u % Q);
-        auto index = [&](int32_t p) { return (int64_t)((it.part + p) * heads + kvh) * R + row; };
+        auto index = [&](int32_t p) { return ((int64_t)(it.part + p) * heads + kvh) * R + row; };
         float m = -INFINITY, sum = 0.f;
         f4 x = {0.f, 0.f, 0.f, 0.f};
         for (int32_t p0 = slice; p0 < parts; p0 += 8 * slices) {

@@ -638,7 +638,7 @@ typedef struct aih_kv_scores {
  * A row that sees no token (a position before the first, blocks outside the
  * cache: a table entry outside [0, n_blocks) hides its tokens) gives zeros; what
  * hidden tokens hold has no effect.  Rows of O outside every request stay as
- * they were.  starts, lens and the tables are read on the device, so that a
+ * they were; O must not overlap Q.  starts, lens and the tables are read on the device, so that a
  * captured step replays over growing requests; `rows` (of Q and O) bounds
  * starts, and table_width * block_tokens bounds lens.  Products are formed on
  * the fp16 matrix cores with q and the probabilities split in two (22 bits; the

@@ -337,3 +337,26 @@ def test_many_requests_in_parts_and_prompts(device):
     b = Batch(device, R.E4M3, 8, 2, 64, 16, lens, lens, seed=2)
     assert b.tile_rows() == 64
     b.check()
+
+
+@pytest.mark.parametrize("new", [[1, 3], [50, 70]])
+def test_extreme_arguments(device, new):
+    """A window as large as an int, prefixes outside the request, more rows than tokens beside a prefix."""
+    b = Batch(device, R.INT8, 4, 2, 64, 16, [200, 100], new)
+    plain = b.run()
+    np.testing.assert_array_equal(b.run(window=2 ** 31 - 1, prefix=[-2 ** 31, -5]), plain)
+    b.check(window=2 ** 31 - 1, prefix=[2 ** 31 - 1, 2 ** 31 - 1])
+    b.lens[1] = new[1] - 2          # its first two rows lie before the first token; they see the prefix
+    b.check(window=2 ** 31 - 1, prefix=[0, 1])
+
+
+def test_starts_that_overlap(device):
+    """Rows claimed by several requests: nothing outside O and the scratch is touched, and the other rows are right."""
+    b = Batch(device, R.INT8, 4, 2, 64, 16, [3000, 500], [64, 64], behind=64)
+    b.lens, b.tables = b.lens * 40, np.tile(b.tables, (40, 1))
+    good = b.starts.copy()
+    b.starts = np.array([0, 64, 0] * 26 + [0, 0, -5])
+    got = b.run()
+    assert got.shape == (192, 4, 64)
+    assert np.all(got[128:] == -7) or np.isfinite(got).all()
+    b.starts = good
