@@ -317,7 +317,8 @@ struct AppendArgs {
     int64_t ldq;
     const int32_t *positions;
     const float *table;
-    int32_t table_rows, q_heads, q_parts;
+    int32_t table_rows, q_heads;
+    int32_t run_groups, q_groups;   // workgroups of the keys and values, and behind them those that rotate Q
 };
 
 // Two rotation pairs of a row at position p, dimensions d .. d + 3 (d % 4 == 0) of its head.
@@ -402,13 +403,14 @@ __device__ __forceinline__ void append_one(uint8_t *codes, float *scale, float o
     }
 }
 
-// Workgroup (x, y): KV head y and the runs of rows of one block that begin
-// among rows RPW x .. RPW x + RPW - 1; y past the KV heads: the queries of
-// those rows.  A run's values are read twice, for their largest magnitude and
+// Workgroup (head fastest): one KV head and the runs of rows of one block that
+// begin among rpw rows; the last workgroups rotate Q, 1024 units of four values
+// each.  A run's values are read twice, for their largest magnitude and
 // to be rounded; the second time they come from the caches.  Every 16-byte
 // unit of the block belongs to one thread, which reads what it keeps of it
 // (rescaled where the scale grew) and writes it once.  A run of one row, as in
-// a decode step, is done by two waves without LDS (append_one).
+// a decode step, is done by two waves without LDS (append_one), two such runs
+// at a time.
 template <int FMT, int D, bool ROPE>
 __global__ void __launch_bounds__(256, 5)
 append_kernel(AppendArgs a, int rpw)
@@ -418,25 +420,34 @@ append_kernel(AppendArgs a, int rpw)
     __shared__ int32_t row_of[256];      // the row (from the run's first) whose token is at an offset of the block
     __shared__ uint32_t top[2][4];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int64_t r0 = (int64_t)blockIdx.x * rpw;
     auto placed = [&](int64_t r) {   // the position of row r allows it to be stored
         if constexpr (!ROPE) return true;
         const int32_t p = a.positions[r];
         return p >= 0 && p < a.table_rows;
     };
-    if (ROPE && (int)blockIdx.y >= a.heads) {
-        const int per = a.q_heads * NQ;
-        for (int64_t r = r0; r < min(r0 + rpw, a.rows); ++r) {
-            if (!placed(r)) continue;
-            const int32_t p = a.positions[r];
-            for (int i = ((int)blockIdx.y - a.heads) * 256 + tid; i < per; i += a.q_parts * 256) {
-                f4 *q = reinterpret_cast<f4 *>(a.Q + r * a.ldq + 4 * i);
-                *q = rotate<D>(*q, a.table, p, 4 * (i % NQ));
-            }
+    if (ROPE && (int)blockIdx.x >= a.run_groups) {
+        const uint32_t per = (uint32_t)a.q_heads * NQ;   // units of a row
+        const int64_t u0 = (int64_t)((int)blockIdx.x - a.run_groups) * 1024, q0 = u0 / per;
+        const uint32_t rest = (uint32_t)(u0 - q0 * per);
+        f4 x[4], *at[4];
+        int32_t p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = rest + 256 * i + tid;
+            const int64_t r = q0 + u / per;
+            at[i] = nullptr;
+            if (r >= a.rows || !placed(r)) continue;
+            at[i] = reinterpret_cast<f4 *>(a.Q + r * a.ldq) + u % per;
+            p[i] = a.positions[r];
+            x[i] = *at[i];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at[i]) *at[i] = rotate<D>(x[i], a.table, p[i], 4 * (tid % NQ));
         return;
     }
-    const int head = blockIdx.y, bt = 1 << a.shift;
+    const int head = (int)blockIdx.x % a.heads, bt = 1 << a.shift;
+    const int64_t r0 = (int64_t)((int)blockIdx.x / a.heads) * rpw;
     auto block_of = [&](int64_t r) {   // the block of row r, -1 for none
         const int32_t slot = a.slots[min(max(r, (int64_t)0), a.rows - 1)];
         const int32_t b = slot < 0 || r < 0 || r >= a.rows ? -1 : slot >> a.shift;
@@ -446,6 +457,7 @@ append_kernel(AppendArgs a, int rpw)
     // (rpw < 64), and how far the first ones reach.
     const int32_t mine = block_of(r0 - 1 + lane), left = __shfl_up(mine, 1);
     unsigned long long runs = __ballot(lane >= 1 && lane <= rpw && mine >= 0 && mine != left);
+    int pair = 0;   // the two waves that do the next run of one row
     while (runs) {
         const int first = __builtin_ctzll(runs);
         runs &= runs - 1;
@@ -470,11 +482,13 @@ append_kernel(AppendArgs a, int rpw)
         uint8_t *kb = a.k + at * bt * D, *vb = a.v + at * bt * D;
         if (n == 1) {
             const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-            if (w < 2 && placed(r)) {
+            const bool ours = w >> 1 == pair;
+            pair ^= 1;
+            if (ours && placed(r)) {
                 const int o = __builtin_amdgcn_readfirstlane(a.slots[r]) & (bt - 1);
                 f4 x = {0.f, 0.f, 0.f, 0.f};
-                if (4 * lane < D) x = w ? *reinterpret_cast<const f4 *>(V + 4 * lane) : key4(0, 4 * lane);
-                if (w) append_one<FMT, D, false>(vb, a.vs + at, old_v, x, o, bt);
+                if (4 * lane < D) x = w & 1 ? *reinterpret_cast<const f4 *>(V + 4 * lane) : key4(0, 4 * lane);
+                if (w & 1) append_one<FMT, D, false>(vb, a.vs + at, old_v, x, o, bt);
                 else append_one<FMT, D, true>(kb, a.ks + at, old_k, x, o, bt);
             }
             continue;
@@ -612,15 +626,10 @@ read_kernel(const uint8_t *__restrict__ k, const uint8_t *__restrict__ v, const 
 // Up to this many rows a plan's one workgroup also places them; more are
 // placed by a second launch over the whole device.
 constexpr int64_t kPlaceRows = 4096;
-// Up to this many rows every workgroup of an append looks at one row, above
-// at a block's worth, at most 32: a prompt's rows come in runs, and a run is the
-// work of its first row.
-constexpr int64_t kSingleRows = 2048;
-
 template <int FMT, int D>
 void launch_append(const AppendArgs &a, bool rope, int rpw, hipStream_t stream)
 {
-    const dim3 grid((unsigned)((a.rows + rpw - 1) / rpw), (unsigned)(a.heads + (rope ? a.q_parts : 0)));
+    const dim3 grid((unsigned)(a.run_groups + a.q_groups));
     if (rope) hipLaunchKernelGGL((append_kernel<FMT, D, true>), grid, dim3(256), 0, stream, a, rpw);
     else hipLaunchKernelGGL((append_kernel<FMT, D, false>), grid, dim3(256), 0, stream, a, rpw);
 }
@@ -640,9 +649,18 @@ int append(aih_ctx *ctx, const aih_kv_cache *kv, AppendArgs a, bool rope)
     a.heads = kv->n_kv_heads;
     a.n_blocks = kv->n_blocks;
     a.shift = aih_kv::log2_of(kv->block_tokens);
-    a.q_parts = rope ? (int32_t)std::min<int64_t>(8, ((int64_t)a.q_heads * kv->head_dim + 1023) / 1024) : 0;
-    if (a.heads + a.q_parts > 65535) return AIH_E_LIMIT;
-    const int rpw = a.rows <= kSingleRows ? 1 : std::min(kv->block_tokens, 32);
+    // Rows whose runs one workgroup does.  A prompt's runs are long, and the workgroups of all rows but their first would
+    // do nothing; single tokens are a run each, done two at a time.  Append alone, us at 1 / 2 / 4 / 8 / 16 / 32 rows, 8
+    // heads, D = 128, int8, blocks of 16: 64 single tokens 3.9 / 4.3 / 5.5 / 8.4 / 14.4 / 26.0, 200 of them 5.9 / 5.3 / 6.4
+    // / 8.8 / 14.7 / 26.4, 64 x 4 11.5 / 7.5 / 7.0 / 10.7 / 19.0 / 35.4, 200 x 4 27.9 / 16.6 / 11.1 / 13.1 / 22.2 / 37.5, a
+    // prompt of 500 12.0 / 10.6 / 9.0 / 8.5 / 7.8 / 13.0, of 1000 18.6 / 16.7 / 14.8 / 9.4 / 8.8 / 13.2, of 2000 32.6 / 28.6
+    // / 24.6 / 16.1 / 11.0 / 16.4; 18000 rows of prompts in blocks of 32 205 / 155 / 140 / 139 / 75 / 57.
+    const int rpw = (int)std::min<int64_t>(a.rows / 128 + 1, std::min(kv->block_tokens, 32));
+    const int64_t runs = (a.rows + rpw - 1) / rpw * a.heads;
+    const int64_t queries = rope ? (a.rows * a.q_heads * (kv->head_dim / 4) + 1023) / 1024 : 0;
+    if (runs + queries > 0x7FFFFFFF) return AIH_E_LIMIT;
+    a.run_groups = (int32_t)runs;
+    a.q_groups = (int32_t)queries;
     aih_kv::DeviceGuard guard(ctx->device);
     AIH_TRY(guard.status);
     const bool i8 = kv->format == AIH_KV_INT8;
