@@ -309,6 +309,38 @@ def test_append_special_values(device, pool, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [127, 128, 700, 2100])
+@pytest.mark.parametrize("heads,dim,block", [(2, 128, 16), (1, 64, 32), (1, 256, 16)])
+def test_append_mixed_runs(device, pool, fmt, heads, dim, block, rows):
+    """Single tokens, runs of a few, whole blocks and skipped rows side by side, into blocks with and without tokens."""
+    rng = np.random.default_rng(rows + dim)
+    n_blocks = rows + 3
+    ref = R.Cache(fmt, heads, dim, block, n_blocks)
+    p = pool(fmt, heads, dim, block, n_blocks, ref)
+    ids = list(rng.permutation(n_blocks))
+    started = ids[::3]
+    k, v = rows_of(rng, len(started), heads, dim)
+    ref.append(k, v, [b * block for b in started])
+    p.append(k, v, [b * block for b in started])
+    slots = []
+    while len(slots) < rows:
+        n = int(rng.choice([1, 1, 1, 2, 5, block, 0]))
+        if n == 0:
+            slots.append(-1)
+            continue
+        b = ids.pop()
+        first = 1 + int(rng.integers(0, block - n)) if n < block else 0
+        slots += [int(b) * block + first + i for i in range(n)]
+    slots = slots[:rows]
+    k, v = rows_of(rng, rows, heads, dim, 3.0)
+    skipped = np.array(slots) < 0
+    k[skipped], v[skipped] = np.nan, np.inf
+    ref.append(k, v, slots)
+    p.append(k, v, slots)
+    p.check()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_append_quotients_beside_ties(device, pool, fmt):
     """Values whose quotient by the scale lies within an ulp of a tie, for many scales."""
     rng = np.random.default_rng(8)
@@ -335,7 +367,7 @@ def test_append_quotients_beside_ties(device, pool, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("heads,dim,block,rows", [(2, 128, 16, 50), (1, 64, 32, 1), (2, 256, 64, 2200)])
+@pytest.mark.parametrize("heads,dim,block,rows", [(2, 128, 16, 50), (1, 64, 32, 1), (3, 128, 16, 333), (2, 256, 64, 2200)])
 def test_append_rope(device, pool, fmt, heads, dim, block, rows):
     """Bit for bit aih_rope of queries and keys, then aih_kv_append; parts of one projection's rows."""
     L, h, n_heads = nat.lib(), device.handle, 2 * heads
