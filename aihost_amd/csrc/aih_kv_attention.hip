@@ -125,8 +125,8 @@ __device__ __forceinline__ Load load_of(const Args &a, int s)
 }
 
 // Item `idx` of one KV head: parts are numbered request by request, tile by
-// tile (the last, longest one first), split by split; with `joined`, tiles
-// instead.  The longest part: the whole work over the wanted workgroups, so that
+// tile (the last, longest one first), split by split; with `joined`, the tiles
+// that are split instead.  The longest part: the whole work over the wanted workgroups, so that
 // all parts are about as long whatever the requests' lengths; longer where
 // rounding up would make a few parts more than that number, which would run
 // alone after the others.  Every wave of the launch runs this with all lanes.
@@ -167,7 +167,8 @@ __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t he
     for (int base = 0; base < a.n_seqs; base += 64) {
         const Load l = base ? load_of<R>(a, base + lane) : first;
         const int32_t n_split = max(1, (l.keys + len - 1) / len);
-        const int32_t own = joined ? l.tiles : l.tiles * n_split, part_own = n_split > 1 ? l.tiles * n_split : 0;
+        const int32_t part_own = n_split > 1 ? l.tiles * n_split : 0;
+        const int32_t own = !joined ? l.tiles * n_split : n_split > 1 ? l.tiles : 0;
         const int32_t upto = wave_scan(own), part_upto = wave_scan(part_own);
         const unsigned long long past = __ballot(before + upto > idx);
         if (past) {
@@ -920,7 +921,7 @@ join_kernel(Args a, int32_t heads)
     const int tid = threadIdx.x;
     const int32_t kvh = blockIdx.x % heads, sub = blockIdx.x / heads % (R / 16);
     const Item it = find_item<R>(a, blockIdx.x / heads / (R / 16), heads, true);
-    if (!it.ok || it.n_split == 1 || it.part < 0 || ((int64_t)it.part + it.n_split) * heads > a.n_part) return;
+    if (!it.ok || it.part < 0 || ((int64_t)it.part + it.n_split) * heads > a.n_part) return;
     const int32_t left = it.q.n * a.group - (it.tile * R + 16 * sub);   // rows from the first of these on
     if (left <= 0) return;
     const Range all = tile_keys<R>(a, it, view_of(a, it));
@@ -989,6 +990,7 @@ join_kernel(Args a, int32_t heads)
 struct Plan {
     int rows, least;
     int64_t target, tiles, items, parts;   // bounds over one KV head (tiles, items) and over all (parts)
+    int64_t joins;                         // of one KV head: tiles that are split
 };
 
 // Up to this many key tiles are not split: a row tile's own workgroup does them in less time than a second launch takes.
@@ -1030,6 +1032,8 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
     p.items = std::min(p.tiles * most_split, p.tiles + 2 * p.target / heads + 2);
     // a tile that is split has more keys than one part, so its parts are at most twice its keys over the length
     p.parts = most_split <= 1 ? 0 : std::min(p.items * heads, 4 * p.target + 4 * heads);
+    // and there are fewer such tiles than work / length
+    p.joins = std::min(p.tiles, 2 * p.target / heads + 2);
     return p;
 }
 
@@ -1040,7 +1044,7 @@ int64_t ml_floats(const Plan &p) { return (p.parts * p.rows * 2 + kAlign - 1) / 
 template <int FMT, int D, bool MOD>
 int launch(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
 {
-    const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.tiles * heads * (p.rows / 16))), block(256);
+    const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.joins * heads * (p.rows / 16))), block(256);
     constexpr int kWide = D == 256 ? 1 : 2;   // at D = 256 a wave's registers hold one column of 16
     if (p.rows == 16) hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
     else if (p.rows == 64) hipLaunchKernelGGL((prompt_kernel<FMT, D, 1, MOD>), grid, block, 0, ctx->stream, a, heads);
@@ -1124,7 +1128,7 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     const int64_t need = ml_floats(p) + p.parts * p.rows * kv->head_dim;
     if (need && (!scratch || !aih_kv::aligned16(scratch) || scratch_floats < need)) return AIH_E_INVALID;
     if (rows == 0) return AIH_OK;
-    if (std::max(p.items, p.tiles * (p.rows / 16)) * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
+    if (std::max(p.items, p.joins * (p.rows / 16)) * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
     Args a{};
     a.k = static_cast<const uint8_t *>(kv->k);
     a.v = static_cast<const uint8_t *>(kv->v);

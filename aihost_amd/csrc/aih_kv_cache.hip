@@ -242,26 +242,36 @@ struct Format<AIH_KV_INT8> {
     static constexpr float kMost = 127.0f;
     // amax / 127, at least the smallest normal number
     __device__ static __forceinline__ float first_scale(float amax) { return fmaxf(amax / 127.0f, 0x1p-126f); }
-    // The code nearest to x / s, ties to even.  x * inv is within 2^-16 of the
-    // quotient, so c is right or, beside a tie, off by one; r = x - c s is
-    // exact (its bits fit: a multiple of the smaller ulp, at most about s / 2),
-    // and 2 r against s says which.
-    __device__ static __forceinline__ int code(float x, float s, float inv)
+    // The code nearest to x / s, ties to even, from c = rint(x * inv), which is right or, beside a tie, off by one: r = x -
+    // c s is exact (its bits fit: a multiple of the smaller ulp, at most about s / 2), and 2 r against s says which.
+    __device__ static __forceinline__ uint32_t exact(float x, float s, float c)
     {
-        float c = __builtin_rintf(x * inv);
         const float r2 = 2.0f * __builtin_fmaf(-c, s, x);
         const bool odd = ((int)c & 1) != 0;
         if (r2 > s || (r2 == s && odd)) c += 1.0f;
         else if (r2 < -s || (r2 == -s && odd)) c -= 1.0f;
-        return (int)fminf(fmaxf(c, -127.0f), 127.0f);
+        return (uint32_t)(int)fminf(fmaxf(c, -127.0f), 127.0f) & 0xFF;
     }
-    // four codes into a word
+    // Four codes into a word.  t = x * inv is within 2^-16 of the quotient, which is at most 127 (to 2^-17): only where t
+    // lies 2^-15 or less from a tie can its rounding be wrong.  Added to 3 2^22 it is rounded to its code in the low byte.
     __device__ static __forceinline__ uint32_t pack(const float *x, float s, float inv)
     {
-        uint32_t w = 0;
+        constexpr float magic = 12582912.0f;
+        float m[4], off = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= (uint32_t)(code(x[i], s, inv) & 0xFF) << (8 * i);
-        return w;
+        for (int i = 0; i < 4; ++i) {
+            const float t = x[i] * inv;
+            m[i] = t + magic;
+            off = fmaxf(off, fabsf(t - (m[i] - magic)));
+        }
+        if (off >= 0.5f - 0x1p-15f) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w |= exact(x[i], s, m[i] - magic) << (8 * i);
+            return w;
+        }
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(m[1]), __float_as_uint(m[0]), 0x0C0C0400u);
+        return lo | __builtin_amdgcn_perm(__float_as_uint(m[3]), __float_as_uint(m[2]), 0x04000C0Cu);
     }
     // the codes of a word times f = 2^-d, rounded
     __device__ static __forceinline__ uint32_t shrink(uint32_t w, float f)
@@ -651,10 +661,10 @@ int append(aih_ctx *ctx, const aih_kv_cache *kv, AppendArgs a, bool rope)
     a.shift = aih_kv::log2_of(kv->block_tokens);
     // Rows whose runs one workgroup does.  A prompt's runs are long, and the workgroups of all rows but their first would
     // do nothing; single tokens are a run each, done two at a time.  Append alone, us at 1 / 2 / 4 / 8 / 16 / 32 rows, 8
-    // heads, D = 128, int8, blocks of 16: 64 single tokens 3.9 / 4.3 / 5.5 / 8.4 / 14.4 / 26.0, 200 of them 5.9 / 5.3 / 6.4
-    // / 8.8 / 14.7 / 26.4, 64 x 4 11.5 / 7.5 / 7.0 / 10.7 / 19.0 / 35.4, 200 x 4 27.9 / 16.6 / 11.1 / 13.1 / 22.2 / 37.5, a
-    // prompt of 500 12.0 / 10.6 / 9.0 / 8.5 / 7.8 / 13.0, of 1000 18.6 / 16.7 / 14.8 / 9.4 / 8.8 / 13.2, of 2000 32.6 / 28.6
-    // / 24.6 / 16.1 / 11.0 / 16.4; 18000 rows of prompts in blocks of 32 205 / 155 / 140 / 139 / 75 / 57.
+    // heads, D = 128, int8, blocks of 16: 32 single tokens 3.5 / 3.8 / 5.1 / 7.8 / 12.9 / 23.6, 200 of them 5.5 / 5.3 / 6.2
+    // / 8.3 / 13.5 / 24.0, 64 x 4 10.1 / 6.4 / 6.1 / 9.0 / 15.3 / 28.2, 200 x 4 24.9 / 14.8 / 9.9 / 11.2 / 18.2 / 30.4, a
+    // prompt of 500 9.4 / 8.1 / 7.4 / 6.8 / 6.4 / 10.1, of 1000 14.4 / 12.7 / 11.6 / 7.7 / 7.1 / 10.4, of 2000 25.8 / 22.3
+    // / 19.7 / 13.0 / 9.4 / 12.7; 18000 rows of prompts in blocks of 32 177 / 131 / 115 / 116 / 65 / 53.
     const int rpw = (int)std::min<int64_t>(a.rows / 128 + 1, std::min(kv->block_tokens, 32));
     const int64_t runs = (a.rows + rpw - 1) / rpw * a.heads;
     const int64_t queries = rope ? (a.rows * a.q_heads * (kv->head_dim / 4) + 1023) / 1024 : 0;
