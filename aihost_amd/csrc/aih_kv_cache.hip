@@ -441,19 +441,25 @@ append_kernel(AppendArgs a, int rpw)
         const uint32_t rest = (uint32_t)(u0 - q0 * per);
         f4 x[4], *at[4];
         int32_t p[4];
+        bool is[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {   // no branches: all loads are in flight at once
             const uint32_t u = rest + 256 * i + tid;
-            const int64_t r = q0 + u / per;
-            at[i] = nullptr;
-            if (r >= a.rows || !placed(r)) continue;
-            at[i] = reinterpret_cast<f4 *>(a.Q + r * a.ldq) + u % per;
+            const int64_t r = min(q0 + u / per, a.rows - 1);
+            is[i] = q0 + u / per < a.rows;
             p[i] = a.positions[r];
+            at[i] = reinterpret_cast<f4 *>(a.Q + r * a.ldq) + u % per;
             x[i] = *at[i];
         }
 #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = p[i] >= 0 && p[i] < a.table_rows;
+            x[i] = rotate<D>(x[i], a.table, in ? p[i] : 0, 4 * (tid % NQ));
+            is[i] = is[i] && in;
+        }
+#pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (at[i]) *at[i] = rotate<D>(x[i], a.table, p[i], 4 * (tid % NQ));
+            if (is[i]) *at[i] = x[i];
         return;
     }
     const int head = (int)blockIdx.x % a.heads, bt = 1 << a.shift;
