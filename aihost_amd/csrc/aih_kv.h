@@ -33,6 +33,9 @@ private:
     bool changed = false;
 };
 
+constexpr int kMaxHeads = 65535;             // of keys and values, and of queries
+constexpr int64_t kMaxGroups = 0xFFFFFF;     // workgroups of 256 threads of a launch: HIP counts threads in 32 bits
+
 // The sizes of a cache description; the pointers are checked where they are used.
 static inline int check_shape(const aih_kv_cache *kv)
 {
@@ -42,8 +45,8 @@ static inline int check_shape(const aih_kv_cache *kv)
     const int bt = kv->block_tokens;
     if (bt != 16 && bt != 32 && bt != 64 && bt != 128 && bt != 256) return AIH_E_UNSUPPORTED;
     const int64_t tokens = (int64_t)kv->n_blocks * bt;
-    // slots are 32-bit, and so are the indices of 16-token groups
-    if (tokens > 0x7FFFFFFF || tokens / 16 * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
+    // slots are 32-bit, and so are the indices of 16-token groups and of a row's values
+    if (tokens > 0x7FFFFFFF || kv->n_kv_heads > kMaxHeads || tokens / 16 * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
     return AIH_OK;
 }
 

@@ -1091,7 +1091,7 @@ int check_batch(const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n
 {
     if (n_heads <= 0 || rows < 0 || n_seqs <= 0 || table_width <= 0 || n_heads % kv->n_kv_heads) return AIH_E_INVALID;
     if (n_seqs > aih_kv::kMaxSeqs || (int64_t)table_width * kv->block_tokens > 0x7FFFFFFF || rows > 0x7FFFFFFF ||
-        rows * (n_heads / kv->n_kv_heads) > 0x7FFFFF00 || n_heads > 1 << 20)
+        rows * (n_heads / kv->n_kv_heads) > 0x7FFFFF00 || n_heads > aih_kv::kMaxHeads)
         return AIH_E_LIMIT;
     return AIH_OK;
 }
@@ -1140,7 +1140,7 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     const int64_t need = ml_floats(p) + p.parts * p.rows * kv->head_dim;
     if (need && (!scratch || !aih_kv::aligned16(scratch) || scratch_floats < need)) return AIH_E_INVALID;
     if (rows == 0) return AIH_OK;
-    if (std::max(p.items, p.joins * (p.rows / 16)) * kv->n_kv_heads > 0x7FFFFFFF) return AIH_E_LIMIT;
+    if (std::max(p.items, p.joins * (p.rows / 16)) * kv->n_kv_heads > aih_kv::kMaxGroups) return AIH_E_LIMIT;
     Args a{};
     a.k = static_cast<const uint8_t *>(kv->k);
     a.v = static_cast<const uint8_t *>(kv->v);

@@ -547,7 +547,7 @@ int aih_attention_decode_qkv(aih_ctx *ctx, const float *QKV, float *Kc, float *V
 #define AIH_KV_E4M3 1
 typedef struct aih_kv_cache {
     int32_t format;        /* AIH_KV_INT8 or AIH_KV_E4M3                    */
-    int32_t n_kv_heads;
+    int32_t n_kv_heads;    /* at most 65535, and so the query heads     */
     int32_t head_dim;      /* 64, 128 or 256                                */
     int32_t block_tokens;  /* 16, 32, 64, 128 or 256                        */
     int32_t n_blocks;      /* n_blocks * block_tokens < 2^31                */

@@ -169,3 +169,16 @@ def test_attention_refuses_caches():
     # tables too short to be split need no scratch; longer ones do
     assert L.aih_kv_attention_scratch_floats(CTX, ok, 4, 8, 2, 4) == 0
     assert L.aih_kv_attention_scratch_floats(CTX, ok, 4, 8, 2, 4096) > 0
+
+
+def test_sizes_past_a_launch_refused():
+    """More heads than an index of a row's values holds, or more threads than one launch counts."""
+    L, c = nat.lib(), ctypes.byref(cache())
+    assert L.aih_kv_cache_bytes(ctypes.byref(cache(n_kv_heads=65535))) == 8 * 16 * 65535 * 128
+    assert L.aih_kv_cache_bytes(ctypes.byref(cache(n_kv_heads=65536))) == LIM
+    assert L.aih_kv_append(CTX, c, 16, 256, 16, 256, 16, 1 << 30) == LIM
+    assert L.aih_kv_read(CTX, c, 16, 1 << 30, 16, 256, 16, 256) == LIM
+    assert L.aih_kv_append_rope(CTX, c, 16, 1 << 24, 65536, 16, 256, 16, 256, 16, 16, 1, 16, 100) == LIM
+    assert L.aih_kv_append_rope(CTX, c, 16, 1 << 20, 8192, 16, 256, 16, 256, 16, 16, 1 << 17, 16, 100) == LIM
+    assert L.aih_kv_attention(CTX, c, 16, 1 << 24, 16, 1 << 24, 1, 65536, 2, 16, 16, 16, 4, 0.1, None, 16, 1 << 40) == LIM
+    assert L.aih_kv_attention(CTX, c, 16, 512, 16, 512, 1 << 29, 4, 2, 16, 16, 16, 4, 0.1, None, 16, 1 << 40) == LIM
