@@ -431,9 +431,11 @@ __device__ __forceinline__ void append_one(uint8_t *codes, float *scale, float o
 // values in flight.  18000 rows of 8 heads, D = 128, blocks of 32, 184 MB: 52 us
 // for either format, 3.5 TB/s (a large copy reaches 4.8 on the card); one read with
 // the rows held in registers takes 127 of them and 53 us.  With Q of 32
-// heads 774 MB and 204 us, 3.8 TB/s.  One token 3.6 us, a launch.
+// heads 774 MB and 186 us, 4.2 TB/s, at 4 waves a SIMD: fewer rows of Q in flight suit
+// the memory better (at 5 waves 206 us; 1000 single tokens 18.9 against 16.5, smaller
+// calls the same).  One token 3.6 us, a launch.
 template <int FMT, int D, bool ROPE>
-__global__ void __launch_bounds__(256, 5)
+__global__ void __launch_bounds__(256, ROPE ? 3 : 5)
 append_kernel(AppendArgs a, int rpw)
 {
     typedef Format<FMT> F;
