@@ -350,6 +350,15 @@ def test_extreme_arguments(device, new):
     b.check(window=2 ** 31 - 1, prefix=[0, 1])
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,lens,new", [
+    (600, 600, 64, [70, 1, 1100], [1, 1, 1]), (71, 1, 64, [300, 20], [1, 3]), (130, 1, 128, [90], [40]),
+    (258, 86, 64, [1100], [2]), (300, 100, 64, [80], [80]), (7, 7, 256, [1040], [30])])
+def test_odd_and_many_heads(device, fmt, heads, kv, dim, lens, new):
+    """More KV heads than workgroups that a call aims at, groups of more rows than a tile has, primes."""
+    Batch(device, fmt, heads, kv, dim, 16, lens, new, pad=4).check()
+
+
 def test_starts_that_overlap(device):
     """Rows claimed by several requests: nothing outside O and the scratch is touched, and the other rows are right."""
     b = Batch(device, R.INT8, 4, 2, 64, 16, [3000, 500], [64, 64], behind=64)
