@@ -37,8 +37,9 @@
 // Work.  Rows are (token, head of the group) pairs of one KV head, token-major,
 // in tiles of R; each tile's keys are split into parts where the tiles alone
 // would leave CUs idle or where one request is much longer than the others.
-// Every workgroup finds its part from the lengths (find_item), so a captured
-// launch follows the requests as they grow.
+// Every workgroup finds its part from the lengths on the device (find_item, and
+// layout_kernel before it for many requests), so a captured launch follows the requests
+// as they grow.
 
 #include "aih_kv.h"
 
@@ -70,6 +71,7 @@ struct Args {
     const float *slopes;
     const int32_t *prefix;
     float *part, *part_ml;      // partial outputs (rows of D floats) and their (maximum, sum)
+    int32_t *layout;            // where the requests' items begin (layout_kernel), or null
     int32_t rows, heads, group, n_seqs, width, n_blocks, shift, window;
     int32_t target, least;      // workgroups wanted; the fewest tiles of a part
     int32_t n_part;             // partial tiles that fit the scratch
@@ -124,74 +126,178 @@ __device__ __forceinline__ Load load_of(const Args &a, int s)
     return l;
 }
 
-// Item `idx` of one KV head: parts are numbered request by request, tile by
-// tile (the last, longest one first), split by split; with `joined`, the tiles
-// that are split instead.  The longest part: the whole work over the wanted workgroups, so that
-// all parts are about as long whatever the requests' lengths; longer where
+// The longest part, in key tiles: the whole work over the wanted workgroups, so
+// that all parts are about as long whatever the requests' lengths; longer where
 // rounding up would make a few parts more than that number, which would run
-// alone after the others.  Every wave of the launch runs this with all lanes.
-// (The sums are floats: the same in every wave, and they only weigh the parts.)
+// alone after the others.  parts(len): how many there would be.  (The sums are
+// floats: the same in every wave, and they only weigh the parts.)
+template <typename Parts>
+__device__ __forceinline__ int32_t part_length(const Args &a, int32_t heads, float work, float tiles, Parts parts)
+{
+    float want = (float)a.target / (float)heads;
+    // about as many tiles as workgroups wanted, and of different lengths: shorter parts even them out (64 requests of
+    // 512 to 7804 tokens, 512 wanted: 94.7 -> 87.3 us)
+    if (tiles > 0.75f * want) want *= 2.0f;
+    int32_t len = max(a.least, (int32_t)ceilf(work / want));
+    if (tiles < want) {
+        for (int i = 0; i < 4; ++i) {
+            const float n = parts(len);
+            if (n <= want) break;
+            len = max(len + 1, (int32_t)((float)len * n / want));
+        }
+    }
+    return len;
+}
+constexpr int32_t kUnsplit = 1 << 30;   // the length where nothing is split
+constexpr int kScan = 256;              // requests that every wave looks through for itself
+
+// Item k of a request (its tiles from the last, longest one on, split by split;
+// `joined`: its tiles), whose parts begin at `parts`.
+__device__ __forceinline__ Item item_of(const Load &l, int32_t seq, int32_t k, int32_t n_split, int32_t parts, bool joined)
+{
+    Item it;
+    it.n_split = n_split;
+    it.tile = joined ? k : l.tiles - 1 - k / n_split;
+    it.split = joined ? 0 : k % n_split;
+    it.seq = seq;
+    it.part = parts + it.tile * n_split;
+    it.q = l.q;
+    it.ok = true;
+    return it;
+}
+
+// Item `idx` of one KV head: parts are numbered request by request; with
+// `joined`, the tiles that are split instead.  Every wave of the launch runs this
+// with all lanes.  Up to kScan requests it adds up their lengths itself; more
+// have been laid out by layout_kernel, and two rounds of loads find the one.
 template <int R>
 __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t heads, bool joined)
 {
     const int lane = threadIdx.x & 63;
-    const Load first = load_of<R>(a, lane);
-    int32_t len = 1 << 30;   // nothing is split
+    Item none{};
+    none.ok = false;
+    const Load own = load_of<R>(a, lane);   // (before the branch: it is on the way of every small call)
+    if (a.layout) {
+        const int32_t n = a.n_seqs + 1;
+        const int32_t *first = a.layout + 4 + (joined ? 2 * n : 0), *parts = a.layout + 4 + n;
+        int32_t base = 0;
+#pragma unroll
+        for (int step = 64; step; step /= 64) {
+            const int32_t s = base + lane * step;
+            const bool past = s >= n || first[min(s, n - 1)] > idx;
+            base += (63 - __builtin_clzll(~__ballot(past) | 1)) * step;   // the last that is not
+        }
+        const int32_t seq = base;
+        if (seq >= a.n_seqs) return none;
+        const Load l = load_of<R>(a, seq);
+        const int32_t len = a.layout[0], n_split = max(1, (l.keys + len - 1) / len), k = idx - first[seq];
+        if (k < 0 || k >= (joined ? l.tiles : l.tiles * n_split)) return none;
+        return item_of(l, seq, k, n_split, parts[seq], joined);
+    }
+    int32_t len = kUnsplit;
     if (a.n_part) {
-        float work = (float)first.tiles * (float)first.keys, tiles_all = (float)first.tiles;
+        float work = (float)own.tiles * (float)own.keys, tiles = (float)own.tiles;
         for (int base = 64; base < a.n_seqs; base += 64) {
             const Load l = load_of<R>(a, base + lane);
             work += (float)l.tiles * (float)l.keys;
-            tiles_all += (float)l.tiles;
+            tiles += (float)l.tiles;
         }
-        float want = (float)a.target / (float)heads;
-        tiles_all = wave_add(tiles_all);
-        // about as many tiles as workgroups wanted, and of different lengths: shorter parts even them out (64 requests of
-        // 512 to 7804 tokens, 512 wanted: 94.7 -> 87.3 us)
-        if (tiles_all > 0.75f * want) want *= 2.0f;
-        len = max(a.least, (int32_t)ceilf(wave_add(work) / want));
-        if (tiles_all < want) {
-            for (int i = 0; i < 4; ++i) {
-                float n = (float)first.tiles * (float)((first.keys + len - 1) / len);
-                for (int base = 64; base < a.n_seqs; base += 64) {
-                    const Load l = load_of<R>(a, base + lane);
-                    n += (float)l.tiles * (float)((l.keys + len - 1) / len);
-                }
-                n = wave_add(n);
-                if (n <= want) break;
-                len = max(len + 1, (int32_t)((float)len * n / want));
+        len = part_length(a, heads, wave_add(work), wave_add(tiles), [&](int32_t len) {
+            float n = (float)own.tiles * (float)((own.keys + len - 1) / len);
+            for (int base = 64; base < a.n_seqs; base += 64) {
+                const Load l = load_of<R>(a, base + lane);
+                n += (float)l.tiles * (float)((l.keys + len - 1) / len);
             }
-        }
+            return wave_add(n);
+        });
     }
     int32_t before = 0, parts = 0;
     for (int base = 0; base < a.n_seqs; base += 64) {
-        const Load l = base ? load_of<R>(a, base + lane) : first;
-        const int32_t n_split = max(1, (l.keys + len - 1) / len);
-        const int32_t part_own = n_split > 1 ? l.tiles * n_split : 0;
-        const int32_t own = !joined ? l.tiles * n_split : n_split > 1 ? l.tiles : 0;
-        const int32_t upto = wave_scan(own), part_upto = wave_scan(part_own);
+        const Load l = base ? load_of<R>(a, base + lane) : own;
+        const int32_t n_split = max(1, (l.keys + len - 1) / len), part_own = n_split > 1 ? l.tiles * n_split : 0;
+        const int32_t items = !joined ? l.tiles * n_split : n_split > 1 ? l.tiles : 0;
+        const int32_t upto = wave_scan(items), part_upto = wave_scan(part_own);
         const unsigned long long past = __ballot(before + upto > idx);
         if (past) {
             const int at = __builtin_ctzll(past);
-            Item it;
-            const int32_t k = idx - (before + __builtin_amdgcn_readlane(upto - own, at));
-            it.n_split = __builtin_amdgcn_readlane(n_split, at);
-            const int32_t nt = __builtin_amdgcn_readlane(l.tiles, at);
-            it.tile = joined ? k : nt - 1 - k / it.n_split;
-            it.split = joined ? 0 : k % it.n_split;
-            it.seq = base + at;
-            it.part = parts + __builtin_amdgcn_readlane(part_upto - part_own, at) + it.tile * it.n_split;
-            it.q = Seq{__builtin_amdgcn_readlane(l.q.start, at), __builtin_amdgcn_readlane(l.q.n, at),
-                       __builtin_amdgcn_readlane(l.q.len, at)};
-            it.ok = true;
-            return it;
+            auto there = [&](int32_t v) { return __builtin_amdgcn_readlane(v, at); };
+            const Load mine{{there(l.q.start), there(l.q.n), there(l.q.len)}, there(l.tiles), there(l.keys)};
+            return item_of(mine, base + at, idx - (before + there(upto - items)), there(n_split),
+                           parts + there(part_upto - part_own), joined);
         }
         before += __builtin_amdgcn_readlane(upto, 63);
         parts += __builtin_amdgcn_readlane(part_upto, 63);
     }
-    Item none{};
-    none.ok = false;
     return none;
+}
+
+// The layout of more than kScan requests, by one workgroup, four of them a
+// thread: the longest part, and the sums before every request (and over all) of
+// items, of parts and of tiles that are split.  Without it every workgroup would go
+// over all requests: one token each of 130 requests of 300 28.4 us without it, 33.1
+// with it, of 256 50.6 / 55.1 (of 2000 tokens 201 / 203), of 1000 234 / 170, of 4000 1728 / 644.
+template <int R>
+__global__ void __launch_bounds__(1024)
+layout_kernel(Args a, int32_t heads)
+{
+    static_assert(aih_kv::kMaxSeqs <= 4 * 1024, "");
+    __shared__ float fs[16];
+    __shared__ int32_t is[3][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    auto add = [&](float v) {
+        v = wave_add(v);
+        __syncthreads();
+        if (lane == 0) fs[w] = v;
+        __syncthreads();
+        float all = 0.f;
+        for (int i = 0; i < 16; ++i) all += fs[i];
+        return all;
+    };
+    Load l[4];
+    float work = 0.f, tiles = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        l[i] = load_of<R>(a, 4 * tid + i);
+        work += (float)l[i].tiles * (float)l[i].keys;
+        tiles += (float)l[i].tiles;
+    }
+    const int32_t len = !a.n_part ? kUnsplit : part_length(a, heads, add(work), add(tiles), [&](int32_t len) {
+        float n = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += (float)l[i].tiles * (float)((l[i].keys + len - 1) / len);
+        return add(n);
+    });
+    int32_t own[4][3], sum[3] = {0, 0, 0}, before[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int32_t n_split = max(1, (l[i].keys + len - 1) / len);
+        own[i][0] = l[i].tiles * n_split;
+        own[i][1] = n_split > 1 ? l[i].tiles * n_split : 0;
+        own[i][2] = n_split > 1 ? l[i].tiles : 0;
+#pragma unroll
+        for (int e = 0; e < 3; ++e) sum[e] += own[i][e];
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+        const int32_t upto = wave_scan(sum[e]);
+        if (lane == 63) is[e][w] = upto;
+        before[e] = upto - sum[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        for (int i = 0; i < w; ++i) before[e] += is[e][i];
+    if (tid == 0) a.layout[0] = len;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = 4 * tid + i;
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+            if (s < a.n_seqs) a.layout[4 + e * (a.n_seqs + 1) + s] = before[e];
+            before[e] += own[i][e];
+            if (s + 1 == a.n_seqs) a.layout[4 + e * (a.n_seqs + 1) + s + 1] = before[e];
+        }
+    }
 }
 
 // What a request's queries see: position p the keys max(0, p - window + 1) ..
@@ -1051,6 +1157,7 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
 
 constexpr int64_t kAlign = 4;   // floats: the partial outputs start on 16 bytes
 
+int64_t layout_floats(int32_t n_seqs) { return n_seqs > kScan ? (4 + 3 * ((int64_t)n_seqs + 1) + kAlign - 1) / kAlign * kAlign : 0; }
 int64_t ml_floats(const Plan &p) { return (p.parts * p.rows * 2 + kAlign - 1) / kAlign * kAlign; }
 
 template <int FMT, int D, bool MOD>
@@ -1058,6 +1165,13 @@ int launch(aih_ctx *ctx, const Args &a, const Plan &p, int32_t heads)
 {
     const dim3 grid((unsigned)(p.items * heads)), join((unsigned)(p.joins * heads * (p.rows / 16))), block(256);
     constexpr int kWide = D == 256 ? 1 : 2;   // at D = 256 a wave's registers hold one column of 16
+    if (a.layout) {
+        if (p.rows == 16) hipLaunchKernelGGL((layout_kernel<16>), dim3(1), dim3(1024), 0, ctx->stream, a, heads);
+        else if (p.rows == 64) hipLaunchKernelGGL((layout_kernel<64>), dim3(1), dim3(1024), 0, ctx->stream, a, heads);
+        else hipLaunchKernelGGL((layout_kernel<64 * kWide>), dim3(1), dim3(1024), 0, ctx->stream, a, heads);
+        const int rc = aih_launch_status();
+        if (rc) return rc;
+    }
     if (p.rows == 16) hipLaunchKernelGGL((few_kernel<FMT, D, MOD>), grid, block, 0, ctx->stream, a, heads);
     else if (p.rows == 64) hipLaunchKernelGGL((prompt_kernel<FMT, D, 1, MOD>), grid, block, 0, ctx->stream, a, heads);
     else hipLaunchKernelGGL((prompt_kernel<FMT, D, kWide, MOD>), grid, block, 0, ctx->stream, a, heads);
@@ -1108,7 +1222,7 @@ int64_t aih_kv_attention_scratch_floats(aih_ctx *ctx, const aih_kv_cache *kv, in
     if (!rc) rc = check_batch(kv, n_heads, rows, n_seqs, table_width);
     if (rc) return rc;
     const Plan p = plan_of(ctx, kv, n_heads, rows, n_seqs, table_width);
-    return ml_floats(p) + p.parts * p.rows * kv->head_dim;
+    return layout_floats(n_seqs) + ml_floats(p) + p.parts * p.rows * kv->head_dim;
 }
 
 int aih_kv_attention_tile_rows(aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_t rows, int32_t n_seqs,
@@ -1137,7 +1251,7 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     if (!scores) scores = &none;
     if (!(scores->cap >= 0.0f) || !std::isfinite(scores->cap) || scores->window < 0) return AIH_E_INVALID;
     const Plan p = plan_of(ctx, kv, n_heads, rows, n_seqs, table_width);
-    const int64_t need = ml_floats(p) + p.parts * p.rows * kv->head_dim;
+    const int64_t before = layout_floats(n_seqs), need = before + ml_floats(p) + p.parts * p.rows * kv->head_dim;
     if (need && (!scratch || !aih_kv::aligned16(scratch) || scratch_floats < need)) return AIH_E_INVALID;
     if (rows == 0) return AIH_OK;
     if (std::max(p.items, p.joins * (p.rows / 16)) * kv->n_kv_heads > aih_kv::kMaxGroups) return AIH_E_LIMIT;
@@ -1155,8 +1269,9 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     a.tables = tables;
     a.slopes = scores->slopes;
     a.prefix = scores->prefix;
-    a.part_ml = scratch;
-    a.part = scratch + ml_floats(p);
+    a.layout = before ? reinterpret_cast<int32_t *>(scratch) : nullptr;
+    a.part_ml = scratch + before;
+    a.part = a.part_ml + ml_floats(p);
     a.rows = (int32_t)rows;
     a.heads = n_heads;
     a.group = n_heads / kv->n_kv_heads;

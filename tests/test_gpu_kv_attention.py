@@ -327,6 +327,19 @@ def test_blocks_that_were_never_started(device, fmt, new):
     np.testing.assert_array_equal(b.run(), plain)
 
 
+@pytest.mark.parametrize("fmt,n,rows", [(R.INT8, 4096, 16), (R.E4M3, 4095, 16), (R.INT8, 65, 16), (R.E4M3, 256, 16), (R.INT8, 257, 16),
+                                        (R.INT8, 300, 64), (R.E4M3, 190, 64)])
+def test_many_requests(device, fmt, n, rows):
+    """As many requests as a call takes, most of a few tokens, some without rows, the first, one inside and the last long
+    enough to be split; prompts of a few rows beside them."""
+    lens = [1 + (5 * s) % 23 for s in range(n)]
+    new = [0 if s % 9 == 4 else 1 if rows == 16 or s % 2 else min(lens[s], 20) for s in range(n)]
+    for s, (length, k) in {0: (2100, 1), n // 2: (3000, 2), n - 1: (1500, 3)}.items():
+        lens[s], new[s] = length, k
+    b = Batch(device, fmt, 4, 1, 64, 32, lens, new, behind=1, seed=n)
+    b.check()
+
+
 def test_many_requests_in_parts_and_prompts(device):
     """More requests than the lanes of a wave: one of them long, so that it is split; prompts in tiles of 64 rows."""
     lens = [5000 if s == 66 else 40 + s for s in range(80)]
