@@ -448,7 +448,6 @@ def _bind(s):
     floats = nat.check_size(L.aih_kv_attention_scratch_floats(h, cache, c["heads"], s.rows, c["seqs"], s.width),
                             "aih_kv_attention_scratch_floats")
     s.scratch = torch.zeros(max(4, floats), device="cuda")
-    torch.cuda.synchronize()
     s.scores = nat.KvScores(cap=s.cap, window=s.window, slopes=s.slopes.data_ptr() if s.slopes is not None else None,
                             prefix=s.prefix.data_ptr() if s.prefix is not None else None)
     row = c["heads"] * c["dim"]
@@ -461,6 +460,9 @@ def _own_run(s):
     calls = s.__dict__.get("calls")
     if calls is None:
         calls = s.calls = _bind(s)
+        # the library has a stream of its own, which does not wait for torch's: what prepare queued has to be there first.
+        # (The outputs are on that stream too; who reads them with torch waits for the device before.)
+        torch.cuda.synchronize()
     for f, a in calls:
         status = f(*a)
         if status:
