@@ -25,14 +25,18 @@
 // Softmax.  In base 2, with the running normalizer, sum and accumulator of each
 // query in the registers of the four lanes that hold it.  A weight is the
 // probability times the value scale, so the normalizer M is taken over both:
-// with t the score and e the exponent of the scale, M is max(t + e) over the keys seen
-// so far, rounded up.  p = 2^(t + e - M) is at most 1, the weight
-// p vs 2^(15 - e) at most 2^15, the accumulator holds O 2^15 2^-M and the
+// with t the score and v the exponent of the scale, M is max(t + v) over the keys seen
+// so far, rounded up.  A lane's exponentials are p = 2^(t + e - M), the weight
+// p vs 2^(15 - e) is at most 2^15, the accumulator holds O 2^15 2^-M and the
 // sum 2^-M of the probabilities' (each p 2^-e).  M and e being integers,
-// rescaling is exact, and rare.  e is held within 60 of the largest exponent that
-// the query has met (a smaller scale's values are below fp32's last bit
-// beside those, and the sum must not lose the probability of a block of zeros),
-// and above -100; blocks that a query does not see do not enter its M.
+// rescaling is exact, and rare.  e is v, but held within 60 of the largest v that
+// the query has met and above -100: the sum must not lose the probability of a
+// block of zeros (no scale, so v is below all) or of tiny values, whose p would
+// underflow.  Into M goes v itself, held above e - 100 and -100: that bounds p
+// and the sum by 2^100 a key, and costs nothing where the scales that a query sees
+// are above 2^-100 and within 2^160 of each other.  Blocks that a query does not see
+// enter neither.  A weight is good to 2^-40 of the largest; a block whose
+// visible codes are all 0 counts for its scale there, as 0 was within half a step of it.
 //
 // Work.  Rows are (token, head of the group) pairs of one KV head, token-major,
 // in tiles of R; each tile's keys are split into parts where the tiles alone
@@ -667,7 +671,7 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const View &v, cons
     }
     const float ve = scale > 0.f && scale < INFINITY ? (float)__builtin_amdgcn_frexp_expf(scale) : kNoExp;
     st.e = fmaxf(st.e, over4_max(ve));
-    const float e = st.e == kNoExp ? 0.f : fmaxf(fmaxf(ve, st.e - 60.f), -100.f);
+    const float e = fmaxf(fmaxf(ve, st.e - 60.f), -100.f), em = fmaxf(fmaxf(ve, e - 100.f), -100.f);
     const float vs = ldexpf(scale, 15 - (int)e);
     float mx = s[0][0];
 #pragma unroll
@@ -684,7 +688,7 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const View &v, cons
             f = 1.0f;
         }
     }
-    const float m = fmaxf(st.m, ceilf(over4_max(fmaf(mx, f, e))));   // f >= 0; a NaN score is left out here and shows below
+    const float m = fmaxf(st.m, ceilf(over4_max(fmaf(mx, f, em))));   // f >= 0; a NaN score is left out here and shows below
     if (__any(m > st.m)) {
         const float back = times2(1.0f, st.m - m);
         st.l *= back;

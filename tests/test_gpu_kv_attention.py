@@ -382,3 +382,51 @@ def test_starts_that_overlap(device):
     assert got.shape == (192, 4, 64)
     assert np.all(got[128:] == -7) or np.isfinite(got).all()
     b.starts = good
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,lens,new,tile,zeros", [
+    (4, 2, 128, [400], [1], 16, 64), (4, 2, 256, [400], [5], 16, 128), (4, 2, 64, [1500], [1], 16, 512),
+    (16, 8, 64, [700], [700], 64, 128), (8, 1, 64, [4000], [1500], 64, 2600), (8, 1, 64, [9000], [1500], 128, 8000)])
+def test_small_values_after_zeros(device, fmt, heads, kv, dim, lens, new, tile, zeros):
+    """Whole key tiles, and a whole part, of blocks without a value scale before values of any size."""
+    b = Batch(device, fmt, heads, kv, dim, 32, lens, new)
+    assert b.tile_rows() == tile
+    t, scales = b.tables[0], b.ref.scales.copy()
+    b.ref.scales[1, t[:zeros // 32]] = 0
+    b.ref.codes[1, t[:zeros // 32]] = 0
+    rows = np.arange(0, new[0], 1 if new[0] < 10 else 83)
+    for f in (1.0, 1e-6, 1e-8, 1e-10, 2.0 ** -60, 2.0 ** -90):
+        b.ref.scales[1, t[zeros // 32:]] = (scales[1, t[zeros // 32:]] * f).astype(np.float32)
+        got = b.run()
+        want, bound = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale, rows=rows)
+        assert within(got[rows], want[rows], bound[rows]), f
+        nrm = np.linalg.norm((got[rows] - want[rows]) / f) / np.linalg.norm(want[rows] / f)
+        assert nrm <= BAR, (f, nrm)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,lens,new,tile", [
+    (4, 2, 128, [400], [1], 16), (4, 2, 64, [1500], [1], 16), (16, 8, 64, [700], [700], 64),
+    (8, 1, 64, [9000], [1500], 128)])
+@pytest.mark.parametrize("small", [2.0 ** -50, 2.0 ** -75, 2.0 ** -100])
+def test_large_values_that_hardly_count(device, fmt, heads, kv, dim, lens, new, tile, small):
+    """The first tokens have values near 1 and scores 130 below the others', whose values are tiny and make the result."""
+    b = Batch(device, fmt, heads, kv, dim, 32, lens, new)
+    assert b.tile_rows() == tile
+    t, n0 = b.tables[0], 128 // 32
+    u = np.where(b.rng.random(dim) < 0.5, -1.0, 1.0)
+    # every score is scale * dim * 16 * key scale * (-1 or 1)
+    b.q[:] = u
+    b.ref.codes[0, t] = 16 * u
+    b.ref.codes[0, t[:n0]] *= -1
+    b.ref.scales[0] = np.float32(65 / (16 * dim * b.scale))
+    b.ref.scales[1, t[:n0]] = np.float32(1.0)
+    b.ref.scales[1, t[n0:]] = (b.ref.scales[1, t[n0:]] * small).astype(np.float32)
+    rows = np.arange(0, new[0], 83)
+    rows = rows[rows + lens[0] - new[0] >= 128]          # those that see a token that counts
+    got = b.run()[rows].astype(np.float64) / small
+    want = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale, rows=rows)[0][rows] / small
+    most = np.abs(b.ref.codes[1, t[n0:]] * b.ref.scales[1, t[n0:], :, None, None]).max() / small
+    # the scores of the tokens that count are equal: sums of n values with 22 bits of a weight, and the weights' sum
+    np.testing.assert_allclose(got, want, rtol=0, atol=most * (2.0 ** -20 + (lens[0] / 32 + 48) * 2.0 ** -23))
