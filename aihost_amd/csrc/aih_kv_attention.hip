@@ -678,14 +678,20 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const View &v, cons
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
-    if constexpr (!MOD) {
-        // beyond 2^20 the rounding of a score is no longer small beside 1: the normalizer and the exponents below have to
-        // come from the same rounded scores
-        if (__any(mx * f > 0x1p20f)) {
+    // Beyond 2^20, of either sign, the rounding of a score is no longer small beside 1: the normalizer and the exponents below
+    // have to come from the same rounded scores (MOD's are rounded already).  Beyond 2^24 the normalizer and the
+    // difference to it are rounded too, as coarsely as the scores: `most` keeps p below 2^(e - em) all the same.
+    float most = INFINITY;
+    if constexpr (MOD) most = (e - em) - mx;
+    else {
+        const bool large = fabsf(mx * f) > 0x1p20f && mx > -INFINITY;   // -inf: the query sees nothing of the group
+        if (__any(large)) {
+            const float by = large ? f : 1.0f;   // (a row's result does not depend on the other rows)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) s[t] *= f;
-            mx *= f;
-            f = 1.0f;
+            for (int t = 0; t < 4; ++t) s[t] *= by;
+            mx *= by;
+            f = large ? 1.0f : f;
+            if (large) most = (e - em) - mx;
         }
     }
     const float m = fmaxf(st.m, ceilf(over4_max(fmaf(mx, f, em))));   // f >= 0; a NaN score is left out here and shows below
@@ -695,7 +701,7 @@ __device__ __forceinline__ Weights score_tile(const Args &a, const View &v, cons
         st.times(back);
         st.m = m;
     }
-    return Weights{f, e - (m == -INFINITY ? 0.f : m), vs, e};
+    return Weights{f, fminf(e - (m == -INFINITY ? 0.f : m), most), vs, e};
 }
 
 // The weights of keys 8 m + 0..7 of the lane's group, split; the sum of their p is added to `sum`.

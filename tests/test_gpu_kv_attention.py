@@ -430,3 +430,31 @@ def test_large_values_that_hardly_count(device, fmt, heads, kv, dim, lens, new, 
     most = np.abs(b.ref.codes[1, t[n0:]] * b.ref.scales[1, t[n0:], :, None, None]).max() / small
     # the scores of the tokens that count are equal: sums of n values with 22 bits of a weight, and the weights' sum
     np.testing.assert_allclose(got, want, rtol=0, atol=most * (2.0 ** -20 + (lens[0] / 32 + 48) * 2.0 ** -23))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,dim,lens,new,tile", [
+    (4, 2, 128, [512], [1], 16), (16, 8, 64, [704], [704], 64), (8, 1, 64, [9024], [1500], 128)])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1.3e7, 2.4e7, 3e8, -1e3, -1e6, -1.3e7, -2.4e7, -3e8])
+@pytest.mark.parametrize("biased", [False, True])
+def test_scores_of_any_size(device, fmt, heads, kv, dim, lens, new, tile, size, biased):
+    """Equal scores, large of either sign, weigh all tokens alike, whatever the values' scale is."""
+    b = Batch(device, fmt, heads, kv, dim, 32, lens, new)
+    assert b.tile_rows() == tile
+    u = np.where(b.rng.random(dim) < 0.5, -1.0, 1.0)
+    b.q[:] = np.sign(size) * u
+    b.ref.codes[0] = 13 * u
+    b.ref.scales[0] = np.float32(abs(size) / (13 * dim * b.scale))
+    rows = np.arange(0, new[0], 83)
+    most = np.abs(b.ref.codes[1]).max()
+    # Every chained sum rounds, relative to the largest value.  Up to 2^20 in base 2 a score is rounded (half a step, to
+    # either side) in tiles of which a row sees a part, and not in others.
+    t = abs(size) / np.log(2)
+    bar = most * (2.0 ** -20 + (lens[0] / 32 + 48) * 2.0 ** -23 + (t * 2.0 ** -23 if t < 2.0 ** 20 else 0))
+    want = None
+    for e in range(4):
+        b.ref.scales[1] = np.float32(0.75 * 2.0 ** -e)     # one for all: see the comment on scores beyond 2^20
+        if want is None:
+            want = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale, rows=rows)[0][rows] / 0.75
+        got = b.run(slopes=[0.0] * heads if biased else None)[rows] / (0.75 * 2.0 ** -e)
+        np.testing.assert_allclose(got, want, rtol=0, atol=bar)
