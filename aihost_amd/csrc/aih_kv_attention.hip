@@ -1295,7 +1295,9 @@ int aih_kv_attention(aih_ctx *ctx, const aih_kv_cache *kv, const float *Q, int64
     a.least = p.least;
     a.n_part = (int32_t)p.parts;
     a.scale = scale;
-    a.cap = scores->cap;
+    // A score divided by the cap must not leave the normal numbers.  2^90 and more cap nothing that 24 bits of a score can
+    // tell apart; below 2^-60 all scores are as good as 0.
+    a.cap = scores->cap > 0.0f ? std::min(std::max(scores->cap, 0x1p-60f), 0x1p90f) : 0.0f;
     aih_kv::DeviceGuard guard(ctx->device);
     AIH_TRY(guard.status);
     return kv->format == AIH_KV_INT8 ? launch_dim<AIH_KV_INT8>(ctx, kv->head_dim, a, p, kv->n_kv_heads)

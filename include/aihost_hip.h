@@ -621,7 +621,7 @@ int aih_kv_read(aih_ctx *ctx, const aih_kv_cache *kv, const int32_t *slots, int6
 
 /* What changes the scores of aih_kv_attention; zeros and NULLs change nothing. */
 typedef struct aih_kv_scores {
-    float          cap;      /* > 0: cap * tanh(score / cap)                       */
+    float          cap;      /* > 0: cap * tanh(score / cap); any positive number   */
     int32_t        window;   /* > 0: only the last `window` tokens, the own included */
     const float   *slopes;   /* n_heads floats, or NULL: - slope * |distance|      */
     const int32_t *prefix;   /* n_seqs ints, or NULL: the first prefix[s] tokens of

@@ -458,3 +458,12 @@ def test_scores_of_any_size(device, fmt, heads, kv, dim, lens, new, tile, size, 
             want = R.attention(b.ref, b.q, b.starts, b.lens, b.tables, b.scale, rows=rows)[0][rows] / 0.75
         got = b.run(slopes=[0.0] * heads if biased else None)[rows] / (0.75 * 2.0 ** -e)
         np.testing.assert_allclose(got, want, rtol=0, atol=bar)
+
+
+@pytest.mark.parametrize("new", [[1], [30], [200]])
+@pytest.mark.parametrize("cap", [3.4028234663852886e38, 1e35, 1e30, 1e-30, 2.0 ** -126, 1e-44])
+def test_caps_of_any_size(device, cap, new):
+    """A cap that no score comes near changes nothing; one below all of them leaves weights that are alike."""
+    b = Batch(device, R.INT8, 4, 2, 128, 16, [300], new)
+    b.ref.codes[0, b.tables[0, 2]] = 0          # scores of 0 among them
+    b.check(cap=cap)
