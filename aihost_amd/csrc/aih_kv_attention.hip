@@ -130,6 +130,14 @@ __device__ __forceinline__ Load load_of(const Args &a, int s)
     return l;
 }
 
+// Row tiles times key tiles (or parts), rounded by itself: every kernel of a call derives the same lengths from the same sums,
+// and a product that the compiler fused into its sum in one of them would not be the same beyond 2^24.
+__device__ __forceinline__ float product(int32_t tiles, int32_t n)
+{
+#pragma clang fp contract(off)
+    return (float)tiles * (float)n;
+}
+
 // The longest part, in key tiles: the whole work over the wanted workgroups, so
 // that all parts are about as long whatever the requests' lengths; longer where
 // rounding up would make a few parts more than that number, which would run
@@ -200,17 +208,17 @@ __device__ __forceinline__ Item find_item(const Args &a, int32_t idx, int32_t he
     }
     int32_t len = kUnsplit;
     if (a.n_part) {
-        float work = (float)own.tiles * (float)own.keys, tiles = (float)own.tiles;
+        float work = product(own.tiles, own.keys), tiles = (float)own.tiles;
         for (int base = 64; base < a.n_seqs; base += 64) {
             const Load l = load_of<R>(a, base + lane);
-            work += (float)l.tiles * (float)l.keys;
+            work += product(l.tiles, l.keys);
             tiles += (float)l.tiles;
         }
         len = part_length(a, heads, wave_add(work), wave_add(tiles), [&](int32_t len) {
-            float n = (float)own.tiles * (float)((own.keys + len - 1) / len);
+            float n = product(own.tiles, (own.keys + len - 1) / len);
             for (int base = 64; base < a.n_seqs; base += 64) {
                 const Load l = load_of<R>(a, base + lane);
-                n += (float)l.tiles * (float)((l.keys + len - 1) / len);
+                n += product(l.tiles, (l.keys + len - 1) / len);
             }
             return wave_add(n);
         });
@@ -262,13 +270,13 @@ layout_kernel(Args a, int32_t heads)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         l[i] = load_of<R>(a, 4 * tid + i);
-        work += (float)l[i].tiles * (float)l[i].keys;
+        work += product(l[i].tiles, l[i].keys);
         tiles += (float)l[i].tiles;
     }
     const int32_t len = !a.n_part ? kUnsplit : part_length(a, heads, add(work), add(tiles), [&](int32_t len) {
         float n = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += (float)l[i].tiles * (float)((l[i].keys + len - 1) / len);
+        for (int i = 0; i < 4; ++i) n += product(l[i].tiles, (l[i].keys + len - 1) / len);
         return add(n);
     });
     int32_t own[4][3], sum[3] = {0, 0, 0}, before[3];

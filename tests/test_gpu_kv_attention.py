@@ -467,3 +467,24 @@ def test_caps_of_any_size(device, cap, new):
     b = Batch(device, R.INT8, 4, 2, 128, 16, [300], new)
     b.ref.codes[0, b.tables[0, 2]] = 0          # scores of 0 among them
     b.check(cap=cap)
+
+
+@pytest.mark.parametrize("tokens,fmt", [(2200000, R.INT8), (2111111, R.E4M3)])
+def test_more_work_than_fp32_counts(device, tokens, fmt):
+    """Row tiles times key tiles beyond 2^24, where the sums that split the work are rounded: the join takes the parts that
+    were written.  The table names a few blocks again and again."""
+    heads, dim, block, blocks, n = 8, 64, 32, 40, 8192
+    b = Batch(device, fmt, heads, 1, dim, block, [block * (blocks - 2)], [n], width=-(-tokens // block))
+    b.tables = b.rng.integers(0, blocks, (1, b.width))
+    b.lens = [tokens]
+    assert b.tile_rows() == 128 and -(-n * heads // 128) * -(-tokens // 64) > 2 ** 24
+    got = b.run()
+    keys, vals = (x[:, 0] for x in b.ref.values())
+    slots = (b.tables[0][:, None] * block + np.arange(block)).reshape(-1)
+    for r in (0, 4097, n - 1):
+        seen = np.bincount(slots[:tokens - n + r + 1], minlength=len(keys))
+        t = b.q[r].astype(np.float64) @ keys.T * b.scale                     # (head, slot)
+        w = np.exp(t - t.max(1, keepdims=True)) * seen
+        want = w @ vals / w.sum(1, keepdims=True)
+        # the sums are chains of an add for 32 keys; all else is far below that
+        np.testing.assert_allclose(got[r], want, rtol=0, atol=np.abs(vals).max() * (tokens / 32) * 2.0 ** -23)
