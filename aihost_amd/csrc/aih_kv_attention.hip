@@ -488,30 +488,24 @@ __device__ __forceinline__ Col column(const Args &a, const Item &it, const Place
     return c;
 }
 
-// Key tiles by what the queries of 16 columns see of them: all of them see
-// all keys of tiles all_lo .. all_hi - 1, some of them some keys of tiles any_lo .. any_hi - 1.
+// The key tiles of which the queries of 16 columns all see all keys: all_lo .. all_hi - 1.
 struct Sight {
-    int32_t all_lo, all_hi, any_lo, any_hi;
+    int32_t all_lo, all_hi;
 };
 
 __device__ __forceinline__ Sight sight_of(const View &v, const Col &c)
 {
     const bool is = c.pos != kNobody;
-    int32_t lo0 = is ? v.lo(c.pos) : 0, lo1 = is ? lo0 : 0x7FFFFFFF;   // largest and smallest
-    int32_t hi0 = is ? v.hi(c.pos) : 0x7FFFFFFF, hi1 = is ? hi0 : 0;   // smallest and largest
+    int32_t lo = is ? v.lo(c.pos) : 0, hi = is ? v.hi(c.pos) : 0x7FFFFFFF;   // the largest, the smallest
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) {
-        lo0 = max(lo0, __shfl_xor(lo0, d));
-        lo1 = min(lo1, __shfl_xor(lo1, d));
-        hi0 = min(hi0, __shfl_xor(hi0, d));
-        hi1 = max(hi1, __shfl_xor(hi1, d));
+        lo = max(lo, __shfl_xor(lo, d));
+        hi = min(hi, __shfl_xor(hi, d));
     }
-    lo0 = __builtin_amdgcn_readfirstlane(lo0);
-    lo1 = __builtin_amdgcn_readfirstlane(lo1);
-    hi0 = __builtin_amdgcn_readfirstlane(hi0);
-    hi1 = __builtin_amdgcn_readfirstlane(hi1);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
     // hi may be 0 or less for a query that sees nothing
-    return Sight{(int32_t)(((uint32_t)lo0 + 63) / 64), hi0 > 0 ? hi0 / 64 : 0, lo1 / 64, hi1 > 0 ? (int32_t)(((uint32_t)hi1 + 63) / 64) : 0};
+    return Sight{(int32_t)(((uint32_t)lo + 63) / 64), hi > 0 ? hi / 64 : 0};
 }
 
 // Q of a column: its loads, and its values split; split() returns the factor
@@ -577,8 +571,8 @@ struct Groups {
 
 __device__ __forceinline__ int32_t load_ids(const Args &a, const Item &it, int32_t t0)
 {
-    const int64_t token = ((int64_t)t0 * 4 + (threadIdx.x & 63)) * 16;
-    return token < it.q.len ? a.tables[(int64_t)it.seq * a.width + (token >> a.shift)] : -1;
+    const uint32_t group = (uint32_t)t0 * 4 + (threadIdx.x & 63);   // of 16 tokens, of the request
+    return group < ((uint32_t)it.q.len + 15) / 16 ? a.tables[(int64_t)it.seq * a.width + (group >> (a.shift - 4))] : -1;
 }
 
 __device__ __forceinline__ Groups load_groups(const Args &a, int32_t id, int32_t kvh, int32_t heads, int32_t t0)
@@ -1000,15 +994,17 @@ prompt_kernel(Args a, int32_t heads)
             }
 #pragma unroll
             for (int n = 0; n < N; ++n) st[n].l += ldexpf(sum[n], -(int)wt[n].e);
-            // the first half's weights, then its products with the second half's weights between them
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 1);
+            // the first half's weights, then its products with the second half's weights between them; three fragments ahead,
+            // or two where cap and slopes take registers (with three D = 128, N = 2 keeps up to 16 bytes in private memory)
+            constexpr int kAhead = MOD ? 2 : 3;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 1);
             __builtin_amdgcn_sched_group_barrier(0x402, 58 * N, 1);
 #pragma unroll
             for (int i = 0; i < 2 * DT; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, N, 1);
                 if (i < DT) __builtin_amdgcn_sched_group_barrier(0x402, 56 * N / (2 * DT), 1);
                 __builtin_amdgcn_sched_group_barrier(0x008, N, 1);
-                if (i + 3 < 2 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+                if (i + kAhead < 2 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
                 if (i < DT) __builtin_amdgcn_sched_group_barrier(0x402, 56 * N / (2 * DT), 1);
             }
         }

@@ -35,3 +35,10 @@ def _private_bytes(src, tmp_path):
 def test_matrix_core_kernels_use_no_private_memory(src, tmp_path):
     used = {k: b for k, b in _private_bytes(src, tmp_path).items() if b}
     assert not used, used
+
+
+@pytest.mark.parametrize("src", ["aih_kv_attention.hip", "aih_kv_cache.hip"])
+def test_kv_cache_kernels_use_no_private_memory(src, tmp_path):
+    """Nor do the paged cache's: their first launch may be in a captured step."""
+    used = {k: b for k, b in _private_bytes(src, tmp_path).items() if b}
+    assert not used, used
