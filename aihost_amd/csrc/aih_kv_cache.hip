@@ -20,9 +20,9 @@ using aih_kv::wave_max;
 using aih_kv::wave_scan;
 
 // ---------------------------------------------------------------- block tables and slot maps
-// Sums of counts that stop at kFull: the largest value they are compared with
-// is a 31-bit count, and a sum that has stopped is above it or equal.  (Stopped
-// addition of non-negative numbers is associative, so it can be scanned.)
+// Sums of counts that stop at kFull, which is above every value that they are
+// compared with (aih_kv_plan refuses larger ones).  (Stopped addition of
+// non-negative numbers is associative, so it can be scanned.)
 constexpr uint32_t kFull = 0x7FFFFFFFu;
 
 __device__ __forceinline__ uint32_t add_full(uint32_t a, uint32_t b) { return min(a + b, kFull); }
@@ -740,7 +740,8 @@ int aih_kv_plan(aih_ctx *ctx, const int32_t *lens, const int32_t *n_new, int32_t
         return AIH_E_INVALID;
     if (block_tokens != 16 && block_tokens != 32 && block_tokens != 64 && block_tokens != 128 && block_tokens != 256)
         return AIH_E_UNSUPPORTED;
-    if (n_seqs > kMaxSeqs || rows > 0x7FFFFFFF || (int64_t)n_blocks * block_tokens > 0x7FFFFFFF ||
+    // (a sum of rows that has stopped at kFull has to be above `rows`)
+    if (n_seqs > kMaxSeqs || rows >= (int64_t)kFull || (int64_t)n_blocks * block_tokens > 0x7FFFFFFF ||
         (int64_t)table_width * block_tokens > 0x7FFFFFFF)
         return AIH_E_LIMIT;
     aih_kv::DeviceGuard guard(ctx->device);

@@ -579,7 +579,7 @@ int64_t aih_kv_cache_bytes(const aih_kv_cache *kv);
  * may be lens and new_n_free n_free; where they are other arrays, a plan that
  * is not carried out changes nothing but table entries past the requests'
  * lengths.  A table entry outside [0, n_blocks) gives the slot -1.  n_seqs at
- * most 4096 (AIH_E_LIMIT). */
+ * most 4096, rows at most 2^31 - 2 (AIH_E_LIMIT). */
 int aih_kv_plan(aih_ctx *ctx, const int32_t *lens, const int32_t *n_new, int32_t n_seqs, int32_t *tables,
                 int32_t table_width, int32_t block_tokens, int32_t n_blocks, const int32_t *free_blocks,
                 const int32_t *n_free, int32_t *new_lens, int32_t *new_n_free, int32_t *starts, int32_t *slots,

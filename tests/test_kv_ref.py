@@ -182,3 +182,8 @@ def test_sizes_past_a_launch_refused():
     assert L.aih_kv_append_rope(CTX, c, 16, 1 << 20, 8192, 16, 256, 16, 256, 16, 16, 1 << 17, 16, 100) == LIM
     assert L.aih_kv_attention(CTX, c, 16, 1 << 24, 16, 1 << 24, 1, 65536, 2, 16, 16, 16, 4, 0.1, None, 16, 1 << 40) == LIM
     assert L.aih_kv_attention(CTX, c, 16, 512, 16, 512, 1 << 29, 4, 2, 16, 16, 16, 4, 0.1, None, 16, 1 << 40) == LIM
+
+
+def test_plan_rows_below_the_sums_limit():
+    """Sums of rows stop at 2^31 - 1, which has to be more than `rows`: a batch of more rows would be taken for one that fits."""
+    assert plan(rows=(1 << 31) - 1) == LIM
