@@ -166,6 +166,8 @@ class PagedKvCache:
     def read(self, layer, request):
         """(keys, values) that a layer holds of a request, as fp32 arrays of
         (tokens, n_kv_heads * head_dim) (aih_kv_read; waits for the device)."""
+        if not 0 <= request < self.max_seqs:
+            raise IndexError("request %d (of %d)" % (request, self.max_seqs))
         c = self.caches[layer]
         n, wide = int(self.lengths()[request]), c.n_kv_heads * c.head_dim
         t = self._get(self.tables + 4 * request * self.width, self.width)

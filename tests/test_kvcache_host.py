@@ -1,0 +1,65 @@
+"""PagedKvCache's own checks and bookkeeping, on the CPU: a cache without a
+device, whose buffers are recorded and whose library calls are counted."""
+import numpy as np
+import pytest
+
+from aihost_amd import _native as nat
+from aihost_amd.kvcache import PagedKvCache
+
+
+class Buffer:
+    def __init__(self, nbytes):
+        self.nbytes, self.live = nbytes, True
+
+    def get_pointer(self):
+        return 1 << 20
+
+    def dispose(self):
+        self.live = False
+
+
+class Device:
+    def __init__(self):
+        self.buffers = []
+
+    def create_buffer(self, nbytes):
+        self.buffers.append(Buffer(nbytes))
+        return self.buffers[-1]
+
+
+class Library:
+    """What is called, and a scratch size that depends on the rows alone."""
+
+    def __init__(self):
+        self.calls = []
+
+    def aih_kv_attention_scratch_floats(self, h, kv, n_heads, rows, n_seqs, width):
+        return 1000 * rows
+
+    def __getattr__(self, name):
+        def f(*a):
+            self.calls.append(name)
+            return nat.AIH_OK
+        return f
+
+
+@pytest.fixture
+def cache():
+    c = PagedKvCache.__new__(PagedKvCache)
+    c.dev, c.h, c.L = Device(), None, Library()
+    c.n_layers, c.max_seqs, c.max_len, c.max_rows, c.n_blocks, c.block_tokens, c.width = 1, 4, 100, 512, 16, 32, 4
+    c._bufs, c.caches = [], [nat.KvCache(n_kv_heads=2, head_dim=64)]
+    c.scratch, c.scratch_floats, c.rows = None, 0, 0
+    for name in ("lens", "n_new", "done", "tables", "free_blocks", "n_free", "refused", "starts", "slots", "positions"):
+        setattr(c, name, c._buf(4096))
+    c.dev.buffers.clear()
+    return c
+
+
+@pytest.mark.parametrize("request_", [-1, -4, 4, 1 << 30])
+def test_read_of_a_request_that_is_not_there(cache, request_):
+    """Before the table is read: a request below 0 would be a row before it."""
+    cache.lengths = lambda: np.zeros(4, np.int32)
+    with pytest.raises(IndexError):
+        cache.read(0, request_)
+    assert not cache.L.calls
