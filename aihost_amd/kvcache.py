@@ -94,7 +94,9 @@ class PagedKvCache:
             self.h, ctypes.byref(self.caches[0]), n_heads, int(rows), self.max_seqs, self.width),
             "aih_kv_attention_scratch_floats")
         if floats > self.scratch_floats:
-            # the smaller one stays: captured graphs may still point at it
+            # the smaller one stays, since captured graphs may still point at it: with at least twice the room each time
+            # all of them together are below four times what is needed
+            floats = max(floats, 2 * self.scratch_floats)
             self.scratch, self.scratch_floats = self._buf(4 * floats), floats
 
     # -- a step

@@ -251,7 +251,7 @@ class LlamaDecoder:
             block = 32
             self.paged = PagedKvCache(device, c.n_layers, c.n_kv_heads, c.head_dim, -(-self.max_len // block), 1,
                                       self.max_len, P, kv_format, block)
-            for rows in {1, P}:
+            for rows in (P, 1):      # the larger first: the other needs no more, as a rule
                 self.paged.reserve(c.n_heads, rows)
         cached = c.n_layers if kv_format is None else 0
         self.kc = [buf(self.max_len * c.kv_dim * 4) for _ in range(cached)]

@@ -63,3 +63,19 @@ def test_read_of_a_request_that_is_not_there(cache, request_):
     with pytest.raises(IndexError):
         cache.read(0, request_)
     assert not cache.L.calls
+
+
+def test_scratch_grows_by_doubling(cache):
+    """Steps whose sizes creep up: what is kept for captured graphs stays within four times what is needed."""
+    for rows in range(1, 513):
+        cache.reserve(8, rows)
+        assert cache.scratch_floats >= 1000 * rows
+    held = sum(b.nbytes for b in cache.dev.buffers if b.live)
+    assert held <= 4 * (4 * 1000 * 512) and len(cache.dev.buffers) <= 11
+    cache.reserve(8, 7)                          # a smaller step takes nothing
+    assert len(cache.dev.buffers) <= 11
+
+
+def test_exact_scratch_at_first(cache):
+    cache.reserve(8, 3)
+    assert cache.scratch_floats == 3000 and [b.nbytes for b in cache.dev.buffers] == [12000]
