@@ -190,4 +190,7 @@ class PagedKvCache:
     def dispose(self):
         for b in self._bufs:
             b.dispose()
-        self._bufs = []
+        self._bufs, self.caches = [], []
+        # the library refuses NULL, so that no later call reaches what is freed
+        self.lens = self.n_new = self.done = self.tables = self.free_blocks = self.n_free = self.refused = None
+        self.starts = self.slots = self.positions = self.scratch = None

@@ -1,5 +1,7 @@
 """PagedKvCache's own checks and bookkeeping, on the CPU: a cache without a
 device, whose buffers are recorded and whose library calls are counted."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -79,3 +81,19 @@ def test_scratch_grows_by_doubling(cache):
 def test_exact_scratch_at_first(cache):
     cache.reserve(8, 3)
     assert cache.scratch_floats == 3000 and [b.nbytes for b in cache.dev.buffers] == [12000]
+
+
+def test_nothing_is_reachable_after_dispose(cache):
+    """The library refuses the pointers that are left, as it does those of a disposed buffer."""
+    ctx = ctypes.create_string_buffer(1 << 14)          # refused calls read nothing of it
+    cache.dispose()
+    cache.L, cache.h, cache.rows = nat.lib(), ctypes.addressof(ctx), 1
+    assert not cache.dev.buffers or not any(b.live for b in cache.dev.buffers)
+    for call in (lambda: cache.plan(rows=1), lambda: cache.release(), lambda: cache.release([1]), lambda: cache.reset(),
+                 lambda: cache.lengths()):
+        with pytest.raises(nat.AihError) as e:
+            call()
+        assert e.value.status == nat.AIH_E_INVALID
+    for call in (lambda: cache.append(0, 16, 128, 16, 128), lambda: cache.attention(0, 16, 128, 16, 128, 2, 1.0)):
+        with pytest.raises(IndexError):
+            call()
