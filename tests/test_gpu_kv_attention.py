@@ -488,3 +488,40 @@ def test_more_work_than_fp32_counts(device, tokens, fmt):
         want = w @ vals / w.sum(1, keepdims=True)
         # the sums are chains of an add for 32 keys; all else is far below that
         np.testing.assert_allclose(got[r], want, rtol=0, atol=np.abs(vals).max() * (tokens / 32) * 2.0 ** -23)
+
+
+def test_starts_that_overlap_stay_inside(device):
+    """A request with rows of its own before many that claim the same rows again and again: its rows are right, the rows of
+    no request stay, and nothing beside O and the scratch is written."""
+    lens, new = [3000, 500], [64, 64]
+    b = Batch(device, R.INT8, 4, 2, 64, 16, lens, new, behind=64)
+    b.lens, b.tables = lens * 41, np.tile(b.tables, (41, 1))
+    n = len(b.lens)
+    starts = np.array([128, 192] + [0, 64] * 40 + [0])[:n + 1]
+    L, h, guard = nat.lib(), device.handle, 64
+    k, v = b.ref.packed()
+    bufs = [upload(device, x) for x in (k, v, b.ref.scales[0].astype(np.float32), b.ref.scales[1].astype(np.float32))]
+    c = nat.KvCache(format=b.ref.fmt, n_kv_heads=2, head_dim=64, block_tokens=16, n_blocks=b.ref.n_blocks,
+                    k=bufs[0].get_pointer(), v=bufs[1].get_pointer(), k_scale=bufs[2].get_pointer(),
+                    v_scale=bufs[3].get_pointer())
+    wide, rows = 4 * 64, b.rows
+    floats = nat.check_size(L.aih_kv_attention_scratch_floats(h, ctypes.byref(c), 4, rows, n, b.width), "scratch")
+    assert floats > 0
+    up = [upload(device, x) for x in (b.q, np.full(rows * wide + 2 * guard, -7, np.float32),
+                                      np.full(floats + 2 * guard, -9, np.float32), starts.astype(I32),
+                                      np.asarray(b.lens, I32), b.tables.astype(I32))]
+    nat.check(L.aih_kv_attention(h, ctypes.byref(c), up[0].get_pointer(), wide, up[1].get_pointer() + 4 * guard, wide, rows, 4, n,
+                                 up[3].get_pointer(), up[4].get_pointer(), up[5].get_pointer(), b.width, b.scale, None,
+                                 up[2].get_pointer() + 4 * guard, floats), "aih_kv_attention")
+    device.synchronize()
+    o = up[1].read_range(0, rows * wide + 2 * guard, np.float32)
+    scratch = up[2].read_range(0, floats + 2 * guard, np.float32)
+    for x in bufs + up:
+        x.dispose()
+    for x, value in ((o, -7), (scratch, -9)):
+        assert np.all(x[:guard] == value) and np.all(x[-guard:] == value)
+    got = o[guard:-guard].reshape(rows, 4, 64)
+    assert np.all(got[64:128] == -7)                       # no request has them
+    assert np.isfinite(got).all()
+    want, bound = R.attention(b.ref, b.q, [128, 192], b.lens[:1], b.tables[:1], b.scale)
+    assert within(got[128:192], want[128:192], bound[128:192])
