@@ -525,3 +525,23 @@ def test_starts_that_overlap_stay_inside(device):
     assert np.isfinite(got).all()
     want, bound = R.attention(b.ref, b.q, [128, 192], b.lens[:1], b.tables[:1], b.scale)
     assert within(got[128:192], want[128:192], bound[128:192])
+
+
+@pytest.mark.parametrize("window", [0, 2 ** 30 + 77, 5])
+def test_as_many_tokens_as_a_length_counts(device, window):
+    """A request of nearly 2^31 tokens; its table names three blocks, one for each part of it, whose values differ."""
+    b = Batch(device, R.E4M3, 2, 1, 64, 256, [100], [1], width=2 ** 23 - 1)
+    tokens = b.lens[0] = (2 ** 23 - 1) * 256 - 3
+    b.tables = np.zeros((1, b.width), np.int32)
+    b.tables[0, 2 ** 22:] = 1
+    b.tables[0, -1] = 2
+    values = (-1.0, 1.0, 3.0)
+    for i, v in enumerate(values):
+        b.ref.codes[1, i], b.ref.scales[1, i] = v, 1.0
+    b.q[:] = 0                                         # all tokens weigh alike
+    low = max(0, tokens - window) if window else 0
+    ends = np.clip([2 ** 30, tokens // 256 * 256, tokens], low, None)
+    counts = np.diff(np.concatenate([[low], ends]))
+    want = (counts * values).sum() / counts.sum()
+    # 2048 waves take 16384 tiles each, an add for each of four products to a tile
+    np.testing.assert_allclose(b.run(window=window), want, rtol=0, atol=3 * 5 * 16384 * 2.0 ** -24)
