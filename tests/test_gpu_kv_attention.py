@@ -545,3 +545,35 @@ def test_as_many_tokens_as_a_length_counts(device, window):
     want = (counts * values).sum() / counts.sum()
     # 2048 waves take 16384 tiles each, an add for each of four products to a tile
     np.testing.assert_allclose(b.run(window=window), want, rtol=0, atol=3 * 5 * 16384 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_mixed_batches_over_wide_tables(device, seed):
+    """What a server sends: requests that wait, single tokens, drafts and prompts in one call, over tables of a fixed
+    capacity (which the tile is chosen by), with any scores."""
+    rng = np.random.default_rng(1000 + seed)
+    pick = lambda *a: a[rng.integers(len(a))]
+    fmt, dim, block, kv = pick(*FORMATS), pick(64, 128, 128, 256), pick(16, 32, 64, 256), pick(1, 2, 3)
+    heads = kv * pick(1, 2, 4, 5)
+    lens, new = [], []
+    for _ in range(rng.integers(1, 10)):
+        n = int(pick(0, 1, 1, rng.integers(2, 9), rng.integers(9, 150)))
+        lens.append(n + int(pick(0, rng.integers(0, 40), rng.integers(0, 600))))
+        new.append(n)
+    if seed % 4 == 0:
+        lens.append(int(rng.integers(1100, 2000)))
+        new.append(1)
+    scores = {}
+    if rng.random() < 0.3:
+        scores["cap"] = float(pick(2.0, 30.0))
+    if rng.random() < 0.3:
+        scores["window"] = int(rng.integers(1, 300))
+    if rng.random() < 0.3:
+        scores["slopes"] = [2.0 ** -(1 + h) for h in range(heads)]
+    if rng.random() < 0.3:
+        scores["prefix"] = [int(rng.integers(0, l + 5)) for l in lens]
+    need = max(1, max(-(-l // block) for l in lens))
+    cap = "cap" in scores
+    b = Batch(device, fmt, heads, kv, dim, block, lens, new, width=need + int(pick(0, 3, 8192 // block, 65536 // block)),
+              pad=int(pick(0, 4)), behind=int(pick(0, 1, 200)) + (sum(new) == 0), seed=seed, q_size=4.0 if cap else 1.0)
+    b.check(bar=4 * BAR if cap else BAR, **scores)
