@@ -728,8 +728,9 @@ __device__ __forceinline__ void weigh(const Weights &w, int m, const f4 *s, floa
 // and join through LDS.  Bound by memory where the cache is long: one token of
 // each of 64 requests of 516 to 7804 tokens (32 heads over 8, D = 128, int8) reads
 // 396 MB and takes 83 us, 4.8 TB/s, what a large copy reaches on the card: two such
-// workgroups to a CU with half a tile of loads ahead are enough for that.  One request of 513 tokens: 9.8 us of dependent steps (lengths,
-// table, codes, three tiles, the join of the waves); eight waves 9.9.
+// workgroups to a CU with half a tile of loads ahead are enough for that.  One request of 513 tokens: 10.1 us, where the
+// waves wait for half of their cycles (lengths, table, codes, the join) and issue for 40% of them (three tiles, their
+// conversions and softmax); eight waves 0.2 more.
 template <int FMT, int D, bool MOD>
 __global__ void __launch_bounds__(256)
 few_kernel(Args a, int32_t heads)
@@ -1136,11 +1137,13 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
     const int64_t most_keys = ((int64_t)table_width * kv->block_tokens + 63) / 64;
     auto tiles_of = [&](int r) { return std::min<int64_t>(n_seqs, rows) + rows * group / r; };
     // The tile of a request's rows, by what a call would take with requests of equal rows and full tables (the lengths
-    // are on the device).  Tiles of 16: 0.5 us of a CU for a tile and 64 keys, and 5 us for every further round of
-    // workgroups; of 64: 1.1 us, or 1.25 us one after the other for the keys of a part, and 12 us for a join.  Measured,
-    // 32 heads over 8, D = 128, int8, us of 16 / 64: 64 tokens after 4000 24.1 / 27.3, 100 after 8000 57.4 / 45.8, 300
-    // after 2000 47.2 / 39.7, 16 requests of 16 after 1000 20.6 / 28.3, of 8 after 1000 13.3 / 27.0, 4 prompts of 100
-    // 14.7 / 9.4, 16 of 40 22.4 / 11.4, one of 150 8.5 / 10.2, of 300 14.3 / 13.1, 8 of 32 after 500 15.1 / 19.4.
+    // are on the device): tables much longer than the requests, and prompts beside single tokens, get the tile of another
+    // batch, which is right but slower (a prompt of 512 under a table for 8192 tokens 28.9 us in place of 19.8).
+    // Tiles of 16: 0.5 us of a CU for a tile and 64 keys, and 5 us for every further round of workgroups; of 64: 1.1 us,
+    // or 1.25 us one after the other for the keys of a part, and 12 us for a join.  Measured, 32 heads over 8, D = 128,
+    // int8, us of 16 / 64: 64 tokens after 4000 24.1 / 27.3, 100 after 8000 57.4 / 45.8, 300 after 2000 47.2 / 39.7, 16
+    // requests of 16 after 1000 20.6 / 28.3, of 8 after 1000 13.3 / 27.0, 4 prompts of 100 14.7 / 9.4, 16 of 40 22.4 /
+    // 11.4, one of 150 8.5 / 10.2, of 300 14.3 / 13.1, 8 of 32 after 500 15.1 / 19.4.
     // Tiles of 128 use a converted key twice as often but are fewer and take longer each: us of 64 / 128: prompt of 1024
     // 35.6 / 45.2 (16 tiles of 128 rows and 64 keys a CU), 100 after 8000 45.9 / 48.5 (16), prompt of 2048 90.1 / 90.7
     // (64), of 4096 284 / 260 (256), 200 after 16000 170 / 118 (55).
@@ -1154,7 +1157,8 @@ Plan plan_of(const aih_ctx *ctx, const aih_kv_cache *kv, int32_t n_heads, int64_
     const bool wide = kv->head_dim < 256 && (double)(tiles_of(128) * heads) * keys >= 48 * cu;
     p.rows = us16 < us64 ? 16 : wide ? 128 : 64;
     p.least = 4;
-    // The workgroups that a CU holds: at D = 256 the registers (16 rows) or LDS (64) allow one, else two.  One token each
+    // At D = 256 the registers (16 rows) or LDS (64) allow one workgroup to a CU, at D = 128 two; at D = 64 three or four
+    // would fit, and two are aimed at as well.  One token each
     // of 16 requests of 1033 to 4884 tokens, D = 256: 48.1 us with one wanted a CU, 50.1 with two, 67 with four; one
     // request of 30000 tokens, D = 128: 22.4 with two, 28.4 with four.
     p.target = (kv->head_dim == 256 ? 1 : 2) * cus;

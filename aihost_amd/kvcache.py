@@ -26,9 +26,11 @@ FORMATS = {"int8": nat.KV_INT8, "e4m3": nat.KV_E4M3}
 
 
 class PagedKvCache:
-    """Requests 0 .. max_seqs-1 of up to max_len tokens each over n_blocks
-    blocks of block_tokens tokens; a step has up to max_rows rows.  fmt:
-    "int8" or "e4m3"."""
+    """Requests 0 .. max_seqs-1 of up to max_len tokens each (rounded up to
+    whole blocks: only past that does plan() refuse) over n_blocks blocks of
+    block_tokens tokens; a step has up to max_rows rows.  fmt: "int8" or
+    "e4m3".  One device, one stream: its steps share the scratch of attention()
+    and run one after the other."""
 
     def __init__(self, device, n_layers, n_kv_heads, head_dim, n_blocks, max_seqs, max_len, max_rows, fmt="int8",
                  block_tokens=32):
@@ -87,7 +89,8 @@ class PagedKvCache:
         self.rows = 0
 
     def reserve(self, n_heads, rows):
-        """Scratch for attention() of `n_heads` query heads over `rows` rows.
+        """Scratch for attention() of `n_heads` query heads over `rows` rows
+        (at least twice as much as before when it grows).
         It cannot grow while the stream is being captured: reserve what the
         captured calls need before."""
         floats = nat.check_size(self.L.aih_kv_attention_scratch_floats(
@@ -109,7 +112,9 @@ class PagedKvCache:
     def plan(self, n_new=None, rows=None):
         """aih_kv_plan of the next step, in place; n_new: new tokens of each
         request (None: as set_new left them); rows: the rows that slots,
-        positions and the calls below cover (default: max_rows)."""
+        positions and the calls below cover (default: max_rows; queries of
+        all of them are read, and attention() chooses its tile by their
+        number, so a step of few rows is faster with its own number)."""
         if n_new is not None:
             self.set_new(n_new)
         rows = self.max_rows if rows is None else int(rows)
